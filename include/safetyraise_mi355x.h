@@ -61,9 +61,14 @@ extern "C" {
 #define SAFETYRAISE_MI355X_GATED UINT32_C(0x20)      /* q rows are per-head [q, gate] */
 #define SAFETYRAISE_MI355X_MROPE_INTERLEAVED UINT32_C(0x40)
 #define SAFETYRAISE_MI355X_KEEP_ROWS UINT32_C(0x80) /* gdn_forward: allow gdn_rollback */
+#define SAFETYRAISE_MI355X_OUTPUT_BF16 UINT32_C(0x100) /* bf16 output (attention_tree_forward, kv_gather) */
 
 /* Largest number of sequences one call may carry. */
 #define SAFETYRAISE_MI355X_MAX_BATCH 1024u
+
+/* Most rows of one sequence in a tree call: attention and GDN layers. */
+#define SAFETYRAISE_MI355X_MAX_TREE_ROWS 128u
+#define SAFETYRAISE_MI355X_MAX_GDN_TREE_ROWS 64u
 
 /* ------------------------------------------------------------------------
  * Context helpers (no counterpart in the reference: the v1 calls are
@@ -301,7 +306,7 @@ SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_write(
  * pre-call buffer, which the KEEP_ROWS call only read, and the per-row decay,
  * correction and key that call recorded: one state read and one write, with
  * the element-wise operations of the forward.  Allowed until the sequence's
- * next gdn_forward or gdn_write; repeated calls rebuild from the same
+ * next gdn_forward, gdn_tree_forward or gdn_write; repeated calls rebuild from the same
  * pre-call state.  flags: SAFETYRAISE_MI355X_ASYNC or 0. */
 SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_rollback(
     safetyraise_kernel_context *context, safetyraise_kernel_gdn_pool *pool, uint32_t sequence,
@@ -346,6 +351,130 @@ typedef struct safetyraise_kernel_gdn_args {
 
 SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_forward(
     safetyraise_kernel_context *context, const safetyraise_kernel_gdn_args *args);
+
+/* ------------------------------------------------------------------------
+ * Trees of drafted tokens.  The reference verifies a chain of drafts
+ * (decode_round, src/engine/speculative.rs:201-216); these calls verify a
+ * tree, in which a position may have several candidates, and commit one path
+ * of it.  No counterpart in the reference.
+ *
+ * A call's rows are the tree's tokens, in an order that has every parent
+ * before its children: parents (a host array, one entry per row of the call)
+ * holds the row's parent as an index within its sequence's rows, or -1 for a
+ * child of the last token before the call.  A chain is -1, 0, 1, ...  A
+ * verify round is: attention_tree_forward and gdn_tree_forward on the layers,
+ * kv_compact of the accepted path's rows, gdn_tree_commit of its last row.
+ *
+ * None of the calls below can be captured into a HIP graph (they read and
+ * advance host-side lengths, page lists and state buffers): INVALID_ARGUMENT.
+ * They run on the context's GPU, whichever device is current.
+ * ---------------------------------------------------------------------- */
+
+/* attention_forward (same tensors, flags and errors) for a tree: row r of a
+ * sequence attends to the tokens cached before the call, its own ancestors
+ * and itself.  Every row is appended, row r at the sequence's length + r, so
+ * the caller gives the position of its depth in `positions`, and keeps the
+ * accepted path with kv_compact.  At most MAX_TREE_ROWS rows per sequence.
+ * out is f32, or bf16 with OUTPUT_BF16.  An f32 result carries f32 products
+ * (q in three bf16 parts, probabilities in two, f32 sums); for a bf16 result
+ * q is used in two parts and the probabilities in one, roundings below its
+ * own.  Any head_dim 1..512 and any group of query heads; 64, 128 and 256
+ * take the MFMA kernel. */
+typedef struct safetyraise_kernel_attention_tree_args {
+    uint32_t struct_size;
+    uint32_t reserved; /* 0 */
+    safetyraise_kernel_attention_args attention; /* out: bf16 values with OUTPUT_BF16 */
+    const int32_t *parents;
+} safetyraise_kernel_attention_tree_args;
+
+SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_attention_tree_forward(
+    safetyraise_kernel_context *context, const safetyraise_kernel_attention_tree_args *args);
+
+/* gdn_forward (same tensors and errors) for a tree: row r's conv and state
+ * follow its own ancestors.  The sequences' states do not change; the call
+ * leaves a record per row, from which gdn_tree_commit builds the state after
+ * any of them.  The pool needs keep_rows of at least the rows per sequence;
+ * at most MAX_GDN_TREE_ROWS.  KEEP_ROWS is refused, and the call ends the
+ * sequences' right to gdn_rollback (it shares that call's records). */
+typedef struct safetyraise_kernel_gdn_tree_args {
+    uint32_t struct_size;
+    uint32_t reserved; /* 0 */
+    safetyraise_kernel_gdn_args gdn;
+    const int32_t *parents;
+} safetyraise_kernel_gdn_tree_args;
+
+SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_tree_forward(
+    safetyraise_kernel_context *context, const safetyraise_kernel_gdn_tree_args *args);
+
+/* Sets each sequence's state and conv history to those after row `row` of its
+ * last gdn_tree_forward (the path from the root to that row), or before that
+ * call (-1).  One launch for any number of layers (pools) and sequences.
+ * Always built from the states before the tree, so a sequence can be
+ * committed again to another row, until its next gdn_forward,
+ * gdn_tree_forward or gdn_write.  A (pool, sequence) twice in one call is
+ * refused.  flags: SAFETYRAISE_MI355X_ASYNC or 0. */
+typedef struct safetyraise_kernel_gdn_commit {
+    safetyraise_kernel_gdn_pool *state;
+    uint32_t sequence;
+    int32_t row;
+} safetyraise_kernel_gdn_commit;
+
+SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_tree_commit(
+    safetyraise_kernel_context *context, const safetyraise_kernel_gdn_commit *commits,
+    uint32_t num_commits, uint32_t flags);
+
+/* Device addresses of a sequence's current state [Hv][Dv][Dk] and conv
+ * history [C][K-1] (f32), valid until the next call that changes or closes
+ * the sequence.  Work queued on the context's stream comes before them. */
+SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_view(
+    safetyraise_kernel_context *context, safetyraise_kernel_gdn_pool *pool, uint32_t sequence,
+    const float **out_matrix, const float **out_history);
+
+/* Keeps chosen tokens of a sequence: its first `start` tokens, then the
+ * `count` tokens start + tokens[i] (host array, strictly ascending, each
+ * below the sequence's length - start).
+ * target == source: the sequence itself becomes those tokens.  Otherwise
+ * target is another open sequence of the pool whose contents they replace (a
+ * fork of chosen tokens); source keeps its own.
+ * Whole pages that stay whole at a page boundary are linked, not copied.
+ * Pages shared with other sequences are never written: tokens that move
+ * there go to free pages, OUT_OF_MEMORY (and nothing changed) when there are
+ * too few.  The tokens' values do not change (keys keep the RoPE position
+ * they were written with).  Entries may name many pools (layers) and
+ * sequences; no sequence may be the target of one entry and appear in
+ * another.  flags: SAFETYRAISE_MI355X_ASYNC or 0. */
+typedef struct safetyraise_kernel_kv_keep {
+    safetyraise_kernel_kv_pool *kv;
+    uint32_t source;
+    uint32_t target;
+    uint64_t start;
+    uint64_t count;
+    const uint32_t *tokens; /* NULL only if count is 0 */
+} safetyraise_kernel_kv_keep;
+
+SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_kv_compact(
+    safetyraise_kernel_context *context, const safetyraise_kernel_kv_keep *entries,
+    uint32_t num_entries, uint32_t flags);
+
+/* kv_read for a list of tokens of many sequences and pools into device (or
+ * host) memory: entry by entry, token start + tokens[i] (any order, repeats
+ * allowed; tokens NULL: start, start + 1, ...), rows of [kv_heads][head_dim]
+ * f32, or bf16 with OUTPUT_BF16 (what kv_append takes with INPUT_BF16).
+ * keys and values are 16-byte aligned when on the device; every pool of a
+ * call has the same kv_heads and head_dim.
+ * flags: DEVICE_POINTERS, ASYNC, OUTPUT_BF16. */
+typedef struct safetyraise_kernel_kv_rows {
+    safetyraise_kernel_kv_pool *kv;
+    uint32_t sequence;
+    uint32_t reserved; /* 0 */
+    uint64_t start;
+    uint64_t count;
+    const uint32_t *tokens;
+} safetyraise_kernel_kv_rows;
+
+SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_kv_gather(
+    safetyraise_kernel_context *context, const safetyraise_kernel_kv_rows *entries,
+    uint32_t num_entries, void *keys, void *values, uint32_t flags);
 
 /* ABI v1 linear (safetyraise_kernel_linear, reference header :115-123) with
  * device pointers: input [rows][cols] and output [rows][out_cols] f32 in

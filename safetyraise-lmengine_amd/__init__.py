@@ -20,6 +20,7 @@ from .plugin import (  # noqa: F401
     INPUT_BF16,
     MROPE_INTERLEAVED,
     NORM_OFFSET,
+    OUTPUT_BF16,
     QK_NORM,
     V1_SYMBOLS,
     GdnState,
@@ -28,7 +29,12 @@ from .plugin import (  # noqa: F401
     PluginError,
     Weight,
     attention_forward,
+    attention_tree_forward,
     gdn_forward,
+    gdn_tree_commit,
+    gdn_tree_forward,
+    kv_compact,
+    kv_gather,
     library_path,
     load_library,
 )

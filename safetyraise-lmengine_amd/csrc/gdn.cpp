@@ -105,6 +105,7 @@ SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_create(
     pool->state_par.assign(o.max_sequences, 0);
     pool->kept.assign(o.max_sequences, Pool::kNoKept);
     pool->kept_at.assign(o.max_sequences, 0);
+    pool->trees.resize(o.max_sequences);
     *out_pool = pool;
     return kOk;
 }
@@ -139,6 +140,7 @@ SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_open(
             pool->open[i] = 1;
             pool->parity[i] = 0;
             pool->kept[i] = Pool::kNoKept;
+            pool->trees[i].parents.clear();
             *out_sequence = i;
             return kOk;
         }
@@ -212,6 +214,7 @@ SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_write(
                                        context->stream));
     }
     pool->kept[sequence] = Pool::kNoKept;
+    pool->trees[sequence].parents.clear();
     if (history != nullptr && pool->history_elems() > 0) {
         SR_HIP(context, hipMemcpyAsync(history_ptr(pool, sequence, pool->parity[sequence]), history,
                                        pool->history_elems() * sizeof(float),
@@ -360,6 +363,7 @@ SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_forward(
         if (keep) pool->state_par[q.slot] ^= 1u;
         pool->kept[q.slot] = keep ? q.rows : Pool::kNoKept;
         pool->kept_at[q.slot] = q.rows;
+        pool->trees[q.slot].parents.clear();
     }
     if (!device) {
         SR_HIP(ctx, hipMemcpyAsync(A.out, g.out, out_b, hipMemcpyDeviceToHost, ctx->stream));

@@ -132,6 +132,17 @@ TimerScope::TimerScope(Ctx *ctx) : prev_(t_timer) {
 }
 TimerScope::~TimerScope() { t_timer = prev_; }
 
+DeviceScope::DeviceScope(Ctx *ctx) {
+    int current = -1;
+    if (hipGetDevice(&current) == hipSuccess && current != ctx->device &&
+        hipSetDevice(ctx->device) == hipSuccess) {
+        prev_ = current;
+    }
+}
+DeviceScope::~DeviceScope() {
+    if (prev_ >= 0) (void)hipSetDevice(prev_);
+}
+
 LaunchEvents timed_launch(const char *kernel) {
     KernelTimer *t = t_timer;
     if (t == nullptr) return {};
@@ -246,12 +257,17 @@ SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_destroy_context(
         status = kDeviceError;
     }
     for (DeviceBuffer *b : {&context->staging, &context->partials, &context->rope_scratch,
-                            &context->linear_in, &context->linear_out,
+                            &context->tree, &context->linear_in, &context->linear_out,
                             &context->linear_part}) {
         if (b->ptr != nullptr) (void)hipFree(b->ptr);
     }
     for (const DeviceBuffer &b : context->linear_kept) (void)hipFree(b.ptr);
     if (context->linear_host != nullptr) (void)hipHostFree(context->linear_host);
+    for (UploadSlot &u : context->upload) {
+        if (u.host != nullptr) (void)hipHostFree(u.host);
+        if (u.dev.ptr != nullptr) (void)hipFree(u.dev.ptr);
+        if (u.fetched != nullptr) (void)hipEventDestroy(u.fetched);
+    }
     destroy_timer_events(context->timer);
     if (context->d_error_word != nullptr) (void)hipFree(context->d_error_word);
     if (context->own_stream != nullptr) (void)hipStreamDestroy(context->own_stream);

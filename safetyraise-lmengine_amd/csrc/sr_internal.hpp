@@ -5,6 +5,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <exception>
 #include <string>
 #include <vector>
 
@@ -43,6 +44,18 @@ struct DeviceBuffer {
     void *ptr = nullptr;
     size_t bytes = 0;
 };
+
+// Host words on their way to the device: pinned memory that a kernel fetches, one
+// slot per call in flight (kv_compact.cpp).
+struct UploadSlot {
+    void *host = nullptr;
+    void *host_dev = nullptr;  // its device address
+    size_t bytes = 0;
+    DeviceBuffer dev;
+    hipEvent_t fetched = nullptr;
+    bool pending = false;
+};
+constexpr int kUploadSlots = 4;
 
 // Per-sequence launch metadata (kernel argument, by value).
 struct SeqMeta {
@@ -111,6 +124,7 @@ struct safetyraise_kernel_context {
     sr::DeviceBuffer staging;          // host-pointer mode device copies
     sr::DeviceBuffer partials;         // split-K partial (m, l, o) records
     sr::DeviceBuffer rope_scratch;     // prefill: per-row RoPE cos/sin
+    sr::DeviceBuffer tree;             // tree attention: q operands, ancestor masks
     sr::DeviceBuffer linear_in;        // linear: the host input's device copy
     sr::DeviceBuffer linear_out;       // linear: the output before it goes back
     sr::DeviceBuffer linear_part;      // linear: split x, partial sums of calls that split K
@@ -118,6 +132,8 @@ struct safetyraise_kernel_context {
     // keep their addresses, so they live as long as the context
     bool linear_captured = false;
     std::vector<sr::DeviceBuffer> linear_kept;
+    sr::UploadSlot upload[sr::kUploadSlots];
+    int upload_next = 0;
     // linear: pinned host staging, kLinearHostBytes of input, then of output,
     // and its device address
     void *linear_host = nullptr;
@@ -185,6 +201,13 @@ struct safetyraise_kernel_gdn_pool {
     std::vector<uint32_t> kept;       // rows of the last KEEP_ROWS call, kNoKept if none since
     std::vector<uint32_t> kept_at;    // row of that call the current buffers hold
     static constexpr uint32_t kNoKept = 0xffffffffu;
+    // the tree of a sequence's last gdn_tree_forward (no parents: none since), and
+    // the buffers that hold what was before it
+    struct Tree {
+        std::vector<int32_t> parents;
+        uint32_t state_par = 0, parity = 0;
+    };
+    std::vector<Tree> trees;
     size_t state_elems() const { return (size_t)value_heads * value_dim * key_dim; }
     size_t history_elems() const { return (size_t)channels * (conv_kernel - 1); }
     uint32_t state_buffers() const { return keep_rows > 0 ? 2u : 1u; }
@@ -223,6 +246,34 @@ class TimerScope {
     KernelTimer *prev_;
 };
 
+// Makes the context's GPU the calling thread's current one for the life of the
+// scope.
+class DeviceScope {
+  public:
+    explicit DeviceScope(Ctx *ctx);
+    ~DeviceScope();
+    DeviceScope(const DeviceScope &) = delete;
+    DeviceScope &operator=(const DeviceScope &) = delete;
+
+  private:
+    int prev_ = -1;
+};
+
+// Runs an entry point's body; a C++ exception (an allocation of its lists) becomes
+// a status instead of leaving through the C boundary.
+template <class F>
+int32_t no_throw(Ctx *ctx, F body) noexcept {
+    try {
+        return body();
+    } catch (const std::exception &) {
+        try {
+            return fail(ctx, kNoMemory, "host memory for the call could not be allocated");
+        } catch (const std::exception &) {
+            return kNoMemory;
+        }
+    }
+}
+
 bool checked_mul(uint64_t a, uint64_t b, uint64_t *out);
 int32_t ensure_buffer(Ctx *ctx, DeviceBuffer &buf, size_t bytes, bool zero);
 int32_t finish_call(Ctx *ctx, bool async);  // sync + sticky error check unless async
@@ -251,6 +302,10 @@ struct TableBatch {
 int32_t kv_prepare_append(Ctx *ctx, safetyraise_kernel_kv_pool *pool, uint32_t seq, uint64_t n,
                           TableBatch *batch = nullptr);
 int32_t kv_flush_table(Ctx *ctx, safetyraise_kernel_kv_pool *pool, TableBatch &batch);
+
+// `count` words of a call's description in device memory (*out), valid for work queued
+// on the context's stream after this.
+int32_t upload_words(Ctx *ctx, const uint32_t *words, size_t count, const uint32_t **out);
 
 // ---------------- kernel launchers (defined in the .hip files) ----------------
 hipError_t launch_page_table_set(hipStream_t s, int32_t *table, const uint32_t *idx,
@@ -352,6 +407,36 @@ hipError_t launch_attn_generic(hipStream_t s, const AttnLaunch &a, const SeqMeta
 hipError_t launch_attn_verify(hipStream_t s, const AttnLaunch &a, const SeqMeta *seqs, int nseq,
                               void *rope_scratch, const DecodePlanInput &in, uint64_t record_limit);
 
+// Attention of a tree of drafts (tree_attn.hip): at most 32 sequences and 1024
+// rows per launch, parents as parent + 1 within the sequence (0: a root), in
+// the order of the rows.
+struct TreeLaunch {
+    const safetyraise_kernel_kv_pool *pool;
+    uint32_t flags, heads, kv_heads, head_dim, rotary_dim;
+    float eps;
+    uint32_t mrope[3];
+    const void *q, *k, *v;
+    const float *q_norm, *k_norm;
+    const int32_t *positions;
+    void *out;
+    uint32_t *err_word;
+    const float *rope_denom;  // theta^(2i/rotary_dim), i < rotary_dim / 2
+    // page-table entries that the launch writes (at most kInlineTable)
+    const uint32_t *tbl_idx = nullptr;
+    const int32_t *tbl_val = nullptr;
+    uint32_t tbl_n = 0;
+    void *q_ops = nullptr, *masks = nullptr;  // scratch (tree_scratch)
+    float *records = nullptr;
+};
+struct TreeScratch {
+    size_t q_bytes = 0, mask_bytes = 0, record_bytes = 0;
+};
+constexpr uint32_t kTreeLaunchSeqs = 32, kTreeLaunchRows = 1024;
+TreeScratch tree_scratch(const TreeLaunch &a, const SeqMeta *seqs, int nseq, uint64_t call_rows,
+                         int num_cus);
+hipError_t launch_tree_attn(hipStream_t stream, const TreeLaunch &a, const SeqMeta *seqs, int nseq,
+                            const uint8_t *parents, int num_cus);
+
 struct GdnLaunch {
     const safetyraise_kernel_gdn_pool *pool;
     const void *qkv, *z, *a, *b;
@@ -376,6 +461,29 @@ struct GdnLaunch {
 struct GdnSeq {
     uint32_t slot, rows, row0, parity, state_in, state_out;
 };
+
+// A tree call (gdn_tree.hip): g as for launch_gdn with records, seqs of at most
+// 64 rows; parents as parent + 1 within the sequence (0: a root).
+constexpr int kGdnTreeSeqs = 32;  // per launch
+size_t gdn_tree_scratch_bytes(const safetyraise_kernel_gdn_pool *pool, uint32_t rows);
+hipError_t launch_gdn_tree(hipStream_t stream, const GdnLaunch &g, const GdnSeq *seqs, int nseq,
+                           const uint8_t *parents, float *scratch);
+
+// The state after the rows of `path` (bits, root first), from the state before the
+// tree and the rows' records.
+struct GdnCommitEntry {
+    const float *state_in;
+    float *state_out;
+    const float *hist_in;
+    float *hist_out;
+    const float *records;
+    uint64_t path;
+    uint32_t rec_stride, value_heads, key_heads, key_dim, value_dim, channels, conv_k, unused;
+};
+constexpr uint32_t kGdnCommitInline = 44;  // entries that fit the kernel arguments
+// device: the entries in device memory, or nullptr (count <= kGdnCommitInline)
+hipError_t launch_gdn_tree_commit(hipStream_t stream, const GdnCommitEntry *entries, uint32_t count,
+                                  const GdnCommitEntry *device);
 
 // gdn_rollback_kernel's inputs for one sequence.
 struct GdnRollback {

@@ -1,0 +1,924 @@
+// Attention of a tree of drafted tokens over the paged bf16 cache, for gfx950.
+//
+// Row r of a sequence (context of `ctx` cached tokens, the call's rows appended
+// behind it) sees every context token and its own ancestors anc(r), itself
+// among them:
+//     o_r = sum_j p_j v_j / sum_j p_j,   p_j = 2^(q_r . k_j - m),
+//     j < ctx  or  j - ctx in anc(r),
+// with q scaled by log2(e) / sqrt(D).  Three launches:
+//   tree_prep_kernel     norms and rotates the new rows; k and v go to the
+//                        cache in bf16, q to the scratch in the form that the
+//                        attention kernel's matrix instructions take, and each
+//                        row's ancestors become a 128-bit mask;
+//   tree_attn_kernel     one workgroup per (sequence, KV head, 32..128 query
+//                        vectors, partition of the keys);
+//   tree_combine_kernel  joins the partitions' records (m, l, o), divides,
+//                        applies the output gate.
+// tree_generic_kernel takes the head widths other than 64, 128 and 256.
+#include <algorithm>
+
+#include "sr_device.hpp"
+#include "tree_plan.hpp"
+
+namespace sr {
+
+namespace {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kTreeSeqs = kTreeLaunchSeqs;
+constexpr uint32_t kTreeRows = kTreeLaunchRows;
+
+struct TreeMeta {
+    uint32_t slot, ctx, rows;
+    uint32_t row0;     // first row in the call's tensors
+    uint32_t tile0;    // first q tile of the sequence (attention kernel)
+    uint32_t block0;   // first workgroup (attention kernel)
+    uint32_t record0;  // first record (attention and combine kernels)
+    uint32_t parts;    // partitions of its keys
+};
+
+struct TreeCommon {
+    uint16_t *k_pages;
+    uint16_t *v_pages;
+    const int32_t *page_table;
+    const void *q;       // raw rows (the gate's values)
+    void *q_ops;         // tiles of q operands, or f32 rows for the generic kernel
+    uint4 *masks;        // [rows of the call] ancestors of each row
+    float *records;
+    void *out;
+    uint32_t *err_word;
+    uint64_t num_pages;
+    uint32_t pages_per_seq, log2_page;
+    uint32_t flags, heads, kv_heads, head_dim;
+    uint32_t nseq, part_keys, vectors;  // vectors: query vectors per workgroup
+    TreeMeta meta[kTreeSeqs];
+};
+
+struct PrepParams {
+    TreeCommon c;
+    const void *k;
+    const void *v;
+    const float *q_norm;
+    const float *k_norm;
+    const int32_t *positions;
+    uint32_t rotary_dim, mrope[3];
+    float eps, qscale;
+    uint32_t rows;    // of the launch, from c.meta[0].row0 on
+    uint32_t parts;   // bf16 parts of q: 3, 2, or 0 for f32 rows
+    uint32_t tbl_n;   // page-table entries that the launch writes
+    uint32_t tbl_idx[kInlineTable];
+    int32_t tbl_val[kInlineTable];
+    float denom[kGenericMaxHeadDim / 2];
+    uint8_t parent[kTreeRows];  // parent + 1 within the sequence, 0 for a root
+};
+static_assert(sizeof(PrepParams) <= 4096, "kernel arguments stay within 4 KiB");
+
+constexpr uint32_t kPrepHeads = 4;  // heads of one row per wave
+constexpr uint32_t kPrepDims = kGenericMaxHeadDim / 64;
+
+// The sequence of launch row `r` (rows are numbered from the launch's first).
+__device__ __forceinline__ uint32_t find_row(const TreeCommon &c, uint32_t r) {
+    uint32_t s = 0;
+    while (s + 1 < c.nseq && c.meta[s + 1].row0 - c.meta[0].row0 <= r) ++s;
+    return s;
+}
+
+// One wave per (row, four heads): KV heads first, then query heads.  NI: dims
+// per lane, d = lane + 64 i.
+template <uint32_t NI>
+__global__ void __launch_bounds__(256) tree_prep_kernel(const PrepParams p) {
+    extern __shared__ float xs_all[];
+    const TreeCommon &c = p.c;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t wave = (uint32_t)wave_index();
+    const uint32_t D = c.head_dim;
+    float *xs = xs_all + (size_t)wave * kPrepHeads * D;
+    const uint32_t all = c.kv_heads + c.heads;
+    const uint32_t groups = (all + kPrepHeads - 1) / kPrepHeads;
+    const uint32_t item = blockIdx.x * 4 + wave;
+    if (blockIdx.x == 0) {
+        for (uint32_t i = threadIdx.x; i < p.tbl_n; i += 256) {
+            ((int32_t *)c.page_table)[p.tbl_idx[i]] = p.tbl_val[i];
+        }
+    }
+    if (item >= p.rows * groups) return;
+    const uint32_t r = item / groups, h0 = item % groups * kPrepHeads;
+    const uint32_t s = find_row(c, r);
+    const TreeMeta m = c.meta[s];
+    const uint32_t row = m.row0 + (r - (m.row0 - c.meta[0].row0));
+    const uint32_t sr = row - m.row0;  // row of the sequence
+    const bool bf16_in = (c.flags & SAFETYRAISE_MI355X_INPUT_BF16) != 0;
+    const bool gated = (c.flags & SAFETYRAISE_MI355X_GATED) != 0;
+    const bool norm = (c.flags & SAFETYRAISE_MI355X_QK_NORM) != 0;
+    const float add = (c.flags & SAFETYRAISE_MI355X_NORM_OFFSET) ? 1.0f : 0.0f;
+    const bool interleaved = (c.flags & SAFETYRAISE_MI355X_MROPE_INTERLEAVED) != 0;
+    const size_t hs = gated ? 2 * (size_t)D : D;
+
+    // all of the wave's values are requested before any is used
+    float x[kPrepHeads][NI], v[kPrepHeads][NI];
+#pragma unroll
+    for (uint32_t u = 0; u < kPrepHeads; ++u) {
+        const uint32_t hh = min(h0 + u, all - 1);
+        const bool kv = hh < c.kv_heads;
+        const void *src = kv ? p.k : c.q;
+        const size_t at = kv ? ((size_t)row * c.kv_heads + hh) * D
+                             : ((size_t)row * c.heads + (hh - c.kv_heads)) * hs;
+#pragma unroll
+        for (uint32_t i = 0; i < NI; ++i) {
+            const uint32_t d = min(lane + 64 * i, D - 1);
+            x[u][i] = load_act_nb(src, at + d, bf16_in);
+            v[u][i] = kv ? load_act_nb(p.v, at + d, bf16_in) : 0.0f;
+        }
+    }
+    // the row's page: its entry may be among those that this launch writes
+    const uint32_t tok = m.ctx + sr;
+    const uint32_t entry = m.slot * c.pages_per_seq + (tok >> c.log2_page);
+    int32_t page = c.page_table[entry];
+    for (uint32_t i = 0; i < p.tbl_n; ++i) {
+        if (p.tbl_idx[i] == entry) page = p.tbl_val[i];
+    }
+    if (h0 == 0) {
+        // the ancestors, walked from the row to its root
+        uint32_t w[4] = {0, 0, 0, 0};
+        const uint8_t *parent = p.parent + (m.row0 - c.meta[0].row0);
+        for (uint32_t a = sr + 1; a != 0; a = parent[a - 1]) {
+            const uint32_t b = a - 1;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) w[k] |= (b >> 5) == k ? 1u << (b & 31) : 0u;
+        }
+        if (lane == 0) c.masks[row] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (norm) {
+#pragma unroll
+        for (uint32_t u = 0; u < kPrepHeads; ++u) {
+            const bool kv = h0 + u < c.kv_heads;
+            const float *w = kv ? p.k_norm : p.q_norm;
+            float ss = 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < NI; ++i) {
+                if (lane + 64 * i < D) ss = fmaf(x[u][i], x[u][i], ss);
+            }
+            ss = sum64(ss);
+            const float variance = ss / (float)D;
+            if (!isfinite(variance) && lane == 0) atomicOr(c.err_word, kErrNonFiniteVariance);
+            const float inv = 1.0f / sqrtf(variance + p.eps);
+#pragma unroll
+            for (uint32_t i = 0; i < NI; ++i) {
+                x[u][i] = x[u][i] * inv * (w[min(lane + 64 * i, D - 1)] + add);
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < kPrepHeads; ++u)
+#pragma unroll
+        for (uint32_t i = 0; i < NI; ++i) {
+            if (lane + 64 * i < D) xs[u * D + lane + 64 * i] = x[u][i];
+        }
+    // (LDS operations of one wave are performed in order)
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    // rotate-half over the first rotary_dim dims (math.rs:52-99)
+    const int32_t *pos = p.positions + (size_t)row * 3;
+    const uint32_t half = p.rotary_dim / 2;
+    for (uint32_t i = lane; i < half; i += 64) {
+        const int axis = rope_axis(i, p.mrope, interleaved);
+        float sn, cs;
+        sincosf((float)pos[axis] / p.denom[i], &sn, &cs);
+#pragma unroll
+        for (uint32_t u = 0; u < kPrepHeads; ++u) {
+            const float left = xs[u * D + i], right = xs[u * D + i + half];
+            xs[u * D + i] = left * cs - right * sn;
+            xs[u * D + i + half] = right * cs + left * sn;
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const uint32_t group = c.heads / c.kv_heads;
+    bool finite = true;
+#pragma unroll
+    for (uint32_t u = 0; u < kPrepHeads; ++u) {
+        const uint32_t hh = h0 + u;
+        if (hh >= all) break;
+        const float *y = xs + u * D;
+        if (hh < c.kv_heads) {
+            const size_t base =
+                ((((size_t)hh * c.num_pages + page) << c.log2_page) + (tok & ((1u << c.log2_page) - 1))) * D;
+#pragma unroll
+            for (uint32_t i = 0; i < NI; ++i) {
+                const uint32_t d = lane + 64 * i;
+                if (d >= D) continue;
+                finite = finite && isfinite(y[d]) && isfinite(v[u][i]);
+                c.k_pages[base + d] = f32_to_bf16(y[d]);
+                c.v_pages[base + d] = f32_to_bf16(v[u][i]);
+            }
+            continue;
+        }
+        const uint32_t head = hh - c.kv_heads;
+        if (p.parts == 0) {
+            float *dst = (float *)c.q_ops + ((size_t)(row - c.meta[0].row0) * c.heads + head) * D;
+#pragma unroll
+            for (uint32_t i = 0; i < NI; ++i) {
+                const uint32_t d = lane + 64 * i;
+                if (d < D) dst[d] = y[d] * p.qscale;
+            }
+            continue;
+        }
+        // q operands: tiles of 32 query vectors (vector = row * group + head of
+        // its KV head), [part][step of 16 dims][lane][8], as a lane of the
+        // attention kernel holds them: vector lane & 31, dims 16 step + 8 (lane
+        // >> 5) + 0..7.  The parts sum to q: bf16 keeps 8 bits of it each.
+        const uint32_t kvh = head / group;
+        const uint32_t vec = sr * group + head % group;
+        const uint32_t tiles = (m.rows * group + 31) / 32;
+        const uint32_t steps = D / 16;
+        const size_t tile = m.tile0 + (size_t)kvh * tiles + vec / 32;
+        if (lane < D / 8) {
+            float a[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) a[j] = y[8 * lane + j] * p.qscale;
+            for (uint32_t part = 0; part < p.parts; ++part) {
+                u32x4 w;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    w[j] = pack_bf16x2(a[2 * j], a[2 * j + 1]);
+                    a[2 * j] -= bf16lo(w[j]);
+                    a[2 * j + 1] -= bf16hi(w[j]);
+                }
+                const size_t at = ((tile * p.parts + part) * steps + lane / 2) * 64 +
+                                  ((lane & 1) * 32 + vec % 32);
+                ((u32x4 *)c.q_ops)[at] = w;
+            }
+        }
+    }
+    if (__builtin_amdgcn_ballot_w64(!finite) != 0 && lane == 0) {
+        atomicOr(c.err_word, kErrNonFiniteKv);
+    }
+}
+
+__device__ __forceinline__ bool mask_bit(const uint4 &m, uint32_t b) {
+    const uint32_t w = b < 64 ? (b < 32 ? m.x : m.y) : (b < 96 ? m.z : m.w);
+    return (w >> (b & 31)) & 1u;
+}
+
+__device__ __forceinline__ void store_out(const TreeCommon &c, size_t at, float y) {
+    if (c.flags & SAFETYRAISE_MI355X_OUTPUT_BF16) {
+        ((uint16_t *)c.out)[at] = f32_to_bf16(y);
+    } else {
+        ((float *)c.out)[at] = y;
+    }
+}
+
+// Any head width: one wave per (row, query head) over the visible keys in tiles
+// of 64, a key per lane for the scores and a dim per lane for the sums.
+__global__ void __launch_bounds__(64) tree_generic_kernel(const TreeCommon c) {
+    extern __shared__ float sh[];
+    const uint32_t D = c.head_dim, lane = threadIdx.x;
+    float *qs = sh, *ps = sh + D;
+    const uint32_t head = blockIdx.x, r = blockIdx.y;
+    const uint32_t s = find_row(c, r);
+    const TreeMeta m = c.meta[s];
+    const uint32_t sr = r - (m.row0 - c.meta[0].row0);
+    const size_t row = (size_t)m.row0 + sr;
+    const float *q = (const float *)c.q_ops + ((size_t)r * c.heads + head) * D;
+    for (uint32_t d = lane; d < D; d += 64) qs[d] = q[d];
+    const uint4 mask = c.masks[row];
+    __syncthreads();
+    const uint32_t kvh = head / (c.heads / c.kv_heads);
+    const uint32_t keys = m.ctx + sr + 1;
+    const int32_t *table = c.page_table + (size_t)m.slot * c.pages_per_seq;
+    const uint32_t pmask = (1u << c.log2_page) - 1;
+    auto base = [&](uint32_t t) {
+        return ((((size_t)kvh * c.num_pages + table[t >> c.log2_page]) << c.log2_page) + (t & pmask)) * D;
+    };
+    float m_run = -INFINITY, l_run = 0.0f;
+    float o[kPrepDims] = {};
+    for (uint32_t t0 = 0; t0 < keys; t0 += 64) {
+        const uint32_t j = t0 + lane;
+        float score = -INFINITY;
+        if (j < keys && (j < m.ctx || mask_bit(mask, j - m.ctx))) {
+            const uint16_t *k = c.k_pages + base(j);
+            float dot = 0.0f;
+            for (uint32_t d = 0; d < D; ++d) dot = fmaf(qs[d], bf16_to_f32(k[d]), dot);
+            score = dot;
+        }
+        const float mx = fmaxf(m_run, max64(score));
+        // (no key so far: every weight is 0)
+        const float ref = mx == -INFINITY ? 0.0f : mx;
+        const float prior = exp2f(m_run - ref);
+        const float pj = exp2f(score - ref);
+        l_run = l_run * prior + sum64(pj);
+        m_run = mx;
+        ps[lane] = pj;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < kPrepDims; ++i) o[i] *= prior;
+        const uint32_t n = min(64u, keys - t0);
+        for (uint32_t k = 0; k < n; ++k) {
+            const float pk = ps[k];
+            if (pk == 0.0f) continue;  // wave-uniform: a masked key's value is not read
+            const uint16_t *v = c.v_pages + base(t0 + k);
+#pragma unroll
+            for (uint32_t i = 0; i < kPrepDims; ++i) {
+                const uint32_t d = lane + 64 * i;
+                if (d < D) o[i] = fmaf(pk, bf16_to_f32(v[d]), o[i]);
+            }
+        }
+        __syncthreads();
+    }
+    const bool bf16_in = (c.flags & SAFETYRAISE_MI355X_INPUT_BF16) != 0;
+    const bool gated = (c.flags & SAFETYRAISE_MI355X_GATED) != 0;
+    const size_t gate = (row * c.heads + head) * 2 * (size_t)D + D;
+    const float inv = 1.0f / l_run;
+#pragma unroll
+    for (uint32_t i = 0; i < kPrepDims; ++i) {
+        const uint32_t d = lane + 64 * i;
+        if (d >= D) continue;
+        float y = o[i] * inv;
+        if (gated) y *= ref_sigmoid(load_act(c.q, gate + d, bf16_in));
+        store_out(c, (row * c.heads + head) * D + d, y);
+    }
+}
+
+
+// ---------------------------------------------------------------------------
+// The MFMA kernel: head widths 64, 128 and 256.
+//
+// S^T = K Q^T and O^T += V^T P^T with v_mfma_f32_32x32x16_bf16 on the cache's own
+// bf16 values: keys (dims) are the rows of the accumulators and a lane's column
+// is one query vector, so its maximum takes one exchange between the two halves
+// of the wave, and the probabilities are in the layout of the next product's
+// operand where they are made.  q and p are split into bf16 parts that sum to
+// them (kF32: 24 bits of q, 16 of p; else 16 and 8), products and sums are f32.
+//
+// A workgroup has up to 4 x 32 query vectors and 32 KB stages of kKeys keys: a
+// wave takes one of the vector groups and 32 keys of a stage.  Stages come
+// straight into LDS (global_load_lds, 16 bytes per lane), kStages - 1 ahead, one
+// barrier per stage; a row's 16-byte units are swapped by its index so that the
+// operand reads (ds_read_b128 of K, ds_read_b64_tr_b16 of V) meet no bank twice.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kStages = 4;
+constexpr uint32_t kStageBytes = 32768;
+constexpr float kLazy = 8.0f;  // log2 growth of the maximum before sums are rescaled
+
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+
+template <int D, int VG, bool kF32>
+struct TreeShape {
+    static constexpr int kKeys = 8192 / D;      // keys per stage
+    static constexpr int KG = kKeys / 32;       // waves over the keys of a stage
+    static constexpr int NW = VG * KG;
+    static constexpr int kThreads = 64 * NW;
+    static constexpr int QP = kF32 ? 3 : 2;     // bf16 parts of q
+    static constexpr int PP = kF32 ? 2 : 1;     // of the probabilities
+    static constexpr size_t kLds = kStages * kStageBytes + kTreePageSlots * 4;
+};
+
+__device__ __forceinline__ float half_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+    return fmaxf(__int_as_float(r[0]), __int_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+    return __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+// The unit (16 bytes) at which logical unit u of key row r is stored.
+template <int D>
+__device__ __forceinline__ uint32_t k_unit(uint32_t r, uint32_t u) {
+    return D == 64 ? u ^ ((r >> 1) & 7) : u ^ (r & 15);
+}
+template <int D>
+__device__ __forceinline__ uint32_t v_unit(uint32_t r, uint32_t u) {
+    return D == 64 ? u ^ (((r >> 1) & 1) << 2) : u ^ ((r & 3) << 2);
+}
+
+// Operands of O^T += V^T P^T for keys 16 st .. of a wave's 32: lane (d = lane & 31
+// of a 32-dim tile, h) gets V[16 st + 4 h + {0..3, 8..11}][d] by two transposing
+// reads per tile.  Written out with their wait: the builtin's reads would wait for
+// every stage that is still on its way into LDS.
+template <int NT>
+struct VFrag {
+    uint2 lo[NT], hi[NT];
+    __device__ __forceinline__ bf16x8 get(int t) const {
+        return __builtin_bit_cast(bf16x8, u32x4{lo[t].x, lo[t].y, hi[t].x, hi[t].y});
+    }
+};
+template <int D, int ST>
+__device__ __forceinline__ void read_v(VFrag<4> &f, const uint32_t (&a)[4]) {
+    constexpr int kLo = ST * 16 * D * 2, kHi = kLo + 8 * D * 2;
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %4, %8 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %2, %10 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %6, %10 offset:%13\n\t"
+        "ds_read_b64_tr_b16 %3, %11 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(f.lo[0]), "=&v"(f.lo[1]), "=&v"(f.lo[2]), "=&v"(f.lo[3]), "=&v"(f.hi[0]),
+          "=&v"(f.hi[1]), "=&v"(f.hi[2]), "=&v"(f.hi[3])
+        : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(kLo), "n"(kHi)
+        : "memory");
+}
+template <int D, int ST>
+__device__ __forceinline__ void read_v(VFrag<2> &f, const uint32_t (&a)[2]) {
+    constexpr int kLo = ST * 16 * D * 2, kHi = kLo + 8 * D * 2;
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %2, %4 offset:%7\n\t"
+        "ds_read_b64_tr_b16 %1, %5 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(f.lo[0]), "=&v"(f.lo[1]), "=&v"(f.hi[0]), "=&v"(f.hi[1])
+        : "v"(a[0]), "v"(a[1]), "n"(kLo), "n"(kHi)
+        : "memory");
+}
+
+template <int D, int VG, bool kF32>
+__global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_kernel(const TreeCommon c) {
+    using T = TreeShape<D, VG, kF32>;
+    constexpr int NS = D / 16, NT = D / 32;
+    constexpr int TPG = NT < 4 ? NT : 4;  // 32-dim tiles per group of V reads
+    constexpr int CH = D / 8;             // 16-byte units per row
+    constexpr int RPI = 64 / CH;          // rows per load instruction
+    constexpr int kLoads = 16 / T::NW > 0 ? 16 / T::NW : 1;  // of K, and of V, per wave and stage
+    static_assert(kLoads * T::NW == 16, "a stage's loads are shared out evenly");
+    extern __shared__ __align__(16) unsigned char lds[];
+    int32_t *pids = (int32_t *)(lds + kStages * kStageBytes);
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    const uint32_t wave = (uint32_t)wave_index();
+    const uint32_t vg = wave % VG, kg = wave / VG;
+    uint32_t s = 0;
+    while (s + 1 < c.nseq && c.meta[s + 1].block0 <= blockIdx.x) ++s;
+    const TreeMeta m = c.meta[s];
+    const uint32_t group = c.heads / c.kv_heads;
+    const uint32_t nvec = m.rows * group;
+    const uint32_t slices = (nvec + 32 * VG - 1) / (32 * VG);
+    // blocks of a sequence: groups of 8 (partition, KV head) units, slice by
+    // slice, so that the slices of a unit run on one XCD (block i runs on XCD i
+    // % 8) at about the same time and share its L2
+    const uint32_t units = m.parts * c.kv_heads;
+    const uint32_t at = blockIdx.x - m.block0;
+    const uint32_t unit0 = at / (8 * slices) * 8;
+    const uint32_t width = min(8u, units - unit0);
+    const uint32_t unit = unit0 + (at - unit0 * slices) % width;
+    const uint32_t slice = (at - unit0 * slices) / width;
+    const uint32_t kvh = unit % c.kv_heads;
+    const uint32_t part = unit / c.kv_heads;
+    const uint32_t key_begin = part * c.part_keys;
+    const uint32_t key_end = min(key_begin + c.part_keys, m.ctx + m.rows);  // > key_begin
+    const uint32_t steps = (key_end - key_begin + T::kKeys - 1) / T::kKeys;
+
+    // page ids of the partition
+    const uint32_t lpt = c.log2_page, pmask = (1u << lpt) - 1;
+    const uint32_t first_page = key_begin >> lpt;
+    const uint32_t npages = ((key_end - 1) >> lpt) - first_page + 1;
+    const int32_t *table = c.page_table + (size_t)m.slot * c.pages_per_seq + first_page;
+    for (uint32_t i = tid; i < npages; i += T::kThreads) pids[i] = table[i];
+    __syncthreads();
+
+    // stage k into its buffer: load i of a wave covers rows RPI (wave + NW i) .. of K
+    // and of V.  Rows past the last key load it again: they are masked, and finite.
+    const unsigned char *k_head = (const unsigned char *)c.k_pages + (((size_t)kvh * c.num_pages) << lpt) * (D * 2);
+    const unsigned char *v_head = (const unsigned char *)c.v_pages + (((size_t)kvh * c.num_pages) << lpt) * (D * 2);
+    const uint32_t lrow = lane / CH, lunit = lane % CH;
+    auto issue = [&](uint32_t k) __attribute__((always_inline)) {
+        unsigned char *buf = lds + (k % kStages) * kStageBytes;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t r0 = RPI * (wave + T::NW * i);
+            const uint32_t key0 = key_begin + k * T::kKeys + r0;
+            const uint32_t base = min(key0, (key_end - 1) & ~(uint32_t)(RPI - 1));
+            const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane(pids[(base >> lpt) - first_page]);
+            const uint32_t tok = min(base + lrow, key_end - 1);
+            const size_t row = (((size_t)page << lpt) + (tok & pmask)) * (D * 2);
+            const uint32_t r = r0 + lrow;
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void *)(k_head + row + k_unit<D>(r, lunit) * 16),
+                (__attribute__((address_space(3))) void *)(buf + r0 * (D * 2)), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void *)(v_head + row + v_unit<D>(r, lunit) * 16),
+                (__attribute__((address_space(3))) void *)(buf + kStageBytes / 2 + r0 * (D * 2)), 16, 0, 0);
+        }
+    };
+    // this wave's query vectors (its first one at least exists, or it only loads)
+    const uint32_t col = lane & 31, h = lane >> 5;
+    const uint32_t tiles = (nvec + 31) / 32;
+    const uint32_t tile = slice * VG + vg;
+    const bool live = tile < tiles;
+    const uint32_t vec = min(tile * 32 + col, nvec - 1);
+    const uint32_t row = vec / group;  // of the sequence
+    bf16x8 q[T::QP][NS];
+    {
+        const u32x4 *src = (const u32x4 *)c.q_ops +
+                           (m.tile0 + (size_t)kvh * tiles + min(tile, tiles - 1)) * T::QP * NS * 64 + lane;
+#pragma unroll
+        for (int p = 0; p < T::QP; ++p)
+#pragma unroll
+            for (int st = 0; st < NS; ++st) q[p][st] = __builtin_bit_cast(bf16x8, src[(p * NS + st) * 64]);
+    }
+    const uint4 mask = c.masks[m.row0 + row];
+    const uint64_t mask_lo = ((uint64_t)mask.y << 32) | mask.x, mask_hi = ((uint64_t)mask.w << 32) | mask.z;
+
+    for (uint32_t k = 0; k + 1 < kStages; ++k) {
+        if (k < steps) issue(k);
+    }
+
+    f32x16 o[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t] = f32x16{};
+    float m_run = -INFINITY, l_run = 0.0f;
+    // LDS addresses of V's transposing reads (k-step 0, first four rows)
+    uint32_t v_at[NT];
+    {
+        const uint32_t i16 = lane & 15, g = lane >> 4;
+        const uint32_t r = 4 * (g >> 1) + (i16 >> 2);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const uint32_t u = 4 * t + ((g & 1) << 1) + ((i16 >> 1) & 1);
+            v_at[t] = kStageBytes / 2 + (32 * kg + r) * (D * 2) + v_unit<D>(r, u) * 16 + (i16 & 1) * 8;
+        }
+    }
+    for (uint32_t k = 0; k < steps; ++k) {
+        // this wave's loads of stage k have landed when at most those of the
+        // stages after it are outstanding
+        constexpr int kPer = 2 * kLoads;
+        const uint32_t after = min(steps - 1 - k, kStages - 2);
+        if (after >= 2) __builtin_amdgcn_s_waitcnt(0x0F70 | ((2 * kPer > 63 ? 63 : 2 * kPer) & 15) | (((2 * kPer > 63 ? 63 : 2 * kPer) >> 4) << 14));
+        else if (after == 1) __builtin_amdgcn_s_waitcnt(0x0F70 | (kPer & 15) | ((kPer >> 4) << 14));
+        else __builtin_amdgcn_s_waitcnt(0x0F70);
+        // every wave's loads of stage k have landed, and the buffer of stage k - 1
+        // has been read
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (k + kStages - 1 < steps) issue(k + kStages - 1);
+        const uint32_t key0 = key_begin + k * T::kKeys + 32 * kg;
+        if (!live || key0 >= key_end) continue;
+        const unsigned char *buf = lds + (k % kStages) * kStageBytes;
+        const unsigned char *kt = buf + 32 * kg * (D * 2);
+        f32x16 sacc{};
+#pragma unroll
+        for (int st = 0; st < NS; ++st) {
+            const bf16x8 a = *(const bf16x8 *)(kt + col * (D * 2) + k_unit<D>(col, 2 * st + h) * 16);
+#pragma unroll
+            for (int p = 0; p < T::QP; ++p) sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[p][st], sacc, 0, 0, 0);
+        }
+        if (key0 + 32 > m.ctx) {
+            // bits of the wave's 32 keys: context keys, and the row's ancestors
+            uint32_t w;
+            if (key0 >= m.ctx) {
+                const uint32_t b = key0 - m.ctx;  // < 128
+                const uint64_t lo = b < 64 ? mask_lo : mask_hi, hi = b < 64 ? mask_hi : 0;
+                const uint32_t sh = b & 63;
+                w = (uint32_t)(lo >> sh) | (sh > 32 ? (uint32_t)(hi << (64 - sh)) : 0u);
+            } else {
+                const uint32_t n = m.ctx - key0;  // 1..31 context keys
+                w = ((uint32_t)mask_lo << n) | ((1u << n) - 1);
+            }
+            w >>= 4 * h;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if (!((w >> (8 * (i >> 2) + (i & 3))) & 1u)) sacc[i] = -INFINITY;
+            }
+        }
+        // d = s - reference.  The reference only moves when the maximum outgrows it by
+        // kLazy (or at the first visible key): sums and outputs are the same for any
+        // common shift, and rescaling is rare.  (The maximum is of differences: of
+        // the matrix products themselves it would cost a canonicalisation each.)
+        float ref = m_run == -INFINITY ? 0.0f : m_run;
+        float d[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) d[i] = sacc[i] - ref;
+        float mx = fmaxf(fmaxf(fmaxf(d[0], d[1]), d[2]), fmaxf(fmaxf(d[3], d[4]), d[5]));
+        mx = fmaxf(fmaxf(mx, d[6]), fmaxf(fmaxf(d[7], d[8]), d[9]));
+        mx = fmaxf(fmaxf(mx, d[10]), fmaxf(fmaxf(d[11], d[12]), d[13]));
+        mx = half_max(fmaxf(fmaxf(mx, d[14]), d[15]));
+        const bool move = mx > kLazy || (m_run == -INFINITY && mx > -INFINITY);
+        if (__builtin_amdgcn_ballot_w64(move) != 0) {
+            const float next = move ? ref + mx : m_run;
+            const float scale = move ? __builtin_amdgcn_exp2f(m_run - next) : 1.0f;
+            m_run = next;
+            ref = next == -INFINITY ? 0.0f : next;
+            l_run *= scale;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] *= scale;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) d[i] = sacc[i] - ref;
+        }
+        bf16x8 p[T::PP][2];
+        float sum[4] = {};
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+            u32x4 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float a = __builtin_amdgcn_exp2f(d[8 * st + 2 * j]);
+                const float b = __builtin_amdgcn_exp2f(d[8 * st + 2 * j + 1]);
+                hi[j] = pack_bf16x2(a, b);
+                if constexpr (kF32) {
+                    lo[j] = pack_bf16x2(a - bf16lo(hi[j]), b - bf16hi(hi[j]));
+                    sum[j] += a + b;
+                } else {
+                    // the sum is over the probabilities that the product uses
+                    sum[j] += bf16lo(hi[j]) + bf16hi(hi[j]);
+                }
+            }
+            p[0][st] = __builtin_bit_cast(bf16x8, hi);
+            if constexpr (kF32) p[1][st] = __builtin_bit_cast(bf16x8, lo);
+        }
+        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const uint32_t vbase = (uint32_t)(uintptr_t)(lds_byte *)buf;
+#pragma unroll
+        for (int tg = 0; tg < NT / TPG; ++tg) {
+            uint32_t a[TPG];
+#pragma unroll
+            for (int t = 0; t < TPG; ++t) a[t] = vbase + v_at[tg * TPG + t];
+            VFrag<TPG> f;
+            read_v<D, 0>(f, a);
+#pragma unroll
+            for (int t = 0; t < TPG; ++t)
+#pragma unroll
+                for (int pp = 0; pp < T::PP; ++pp)
+                    o[tg * TPG + t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.get(t), p[pp][0], o[tg * TPG + t], 0, 0, 0);
+            VFrag<TPG> e;
+            read_v<D, 1>(e, a);
+#pragma unroll
+            for (int t = 0; t < TPG; ++t)
+#pragma unroll
+                for (int pp = 0; pp < T::PP; ++pp)
+                    o[tg * TPG + t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e.get(t), p[pp][1], o[tg * TPG + t], 0, 0, 0);
+        }
+    }
+    float l = half_sum(l_run);
+    // join the waves over the keys, through the stages' LDS
+    if constexpr (T::KG > 1) {
+        __syncthreads();
+        float *x = (float *)lds;
+        constexpr uint32_t kWaveFloats = (NT * 16 + 2) * 64;
+        if (kg > 0) {
+            float *w = x + ((kg - 1) * VG + vg) * kWaveFloats + lane;
+            w[0] = m_run;
+            w[64] = l;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) w[(2 + 16 * t + i) * 64] = o[t][i];
+        }
+        __syncthreads();
+        if (kg > 0) return;
+#pragma unroll 1
+        for (int g = 1; g < T::KG; ++g) {
+            const float *w = x + ((g - 1) * VG + vg) * kWaveFloats + lane;
+            const float m2 = w[0], l2 = w[64];
+            const float mx = fmaxf(m_run, m2);
+            const float ref = mx == -INFINITY ? 0.0f : mx;
+            const float s1 = __builtin_amdgcn_exp2f(m_run - ref), s2 = __builtin_amdgcn_exp2f(m2 - ref);
+            m_run = mx;
+            l = l * s1 + l2 * s2;
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[t][i] = o[t][i] * s1 + w[(2 + 16 * t + i) * 64] * s2;
+        }
+    }
+    if (!live || tile * 32 + col >= nvec) return;
+    const uint32_t head = kvh * group + vec % group;
+    const size_t out_row = (size_t)(m.row0 + row) * c.heads + head;
+    if (c.records != nullptr) {
+        float *rec = c.records + ((size_t)m.record0 + ((size_t)row * c.heads + head) * m.parts + part) *
+                                     tree_record_floats(D);
+        if (h == 0) *(float2 *)rec = make_float2(m_run, l);
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+                *(float4 *)(rec + 4 + 32 * t + 8 * a + 4 * h) =
+                    make_float4(o[t][4 * a], o[t][4 * a + 1], o[t][4 * a + 2], o[t][4 * a + 3]);
+        return;
+    }
+    const bool gated = (c.flags & SAFETYRAISE_MI355X_GATED) != 0;
+    const bool bf16_in = (c.flags & SAFETYRAISE_MI355X_INPUT_BF16) != 0;
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const uint32_t d = 32 * t + 8 * a + 4 * h;
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                y[j] = o[t][4 * a + j] * inv;
+                if (gated) y[j] *= ref_sigmoid(load_act(c.q, out_row * 2 * D + D + d + j, bf16_in));
+            }
+            if (c.flags & SAFETYRAISE_MI355X_OUTPUT_BF16) {
+                *(uint2 *)((uint16_t *)c.out + out_row * D + d) =
+                    make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+            } else {
+                *(float4 *)((float *)c.out + out_row * D + d) = make_float4(y[0], y[1], y[2], y[3]);
+            }
+        }
+}
+
+// Joins the records of a (row, head): a wave each, all the loads of eight records
+// in flight.
+template <int D>
+__global__ void __launch_bounds__(256) tree_combine_kernel(const TreeCommon c, uint32_t rows) {
+    constexpr int EPL = D / 64, kBatch = 8;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t w = blockIdx.x * 4 + (uint32_t)wave_index();
+    if (w >= rows * c.heads) return;
+    const uint32_t r = w / c.heads, head = w % c.heads;
+    const uint32_t s = find_row(c, r);
+    const TreeMeta m = c.meta[s];
+    const uint32_t sr = r - (m.row0 - c.meta[0].row0);
+    const float *rec = c.records + ((size_t)m.record0 + ((size_t)sr * c.heads + head) * m.parts) * tree_record_floats(D);
+    float mx = -INFINITY;
+    for (uint32_t i = lane; i < m.parts; i += 64) mx = fmaxf(mx, rec[(size_t)i * tree_record_floats(D)]);
+    mx = max64(mx);  // finite: a row sees itself
+    float l = 0.0f, o[EPL] = {};
+    for (uint32_t i0 = 0; i0 < m.parts; i0 += kBatch) {
+        float2 ml[kBatch];
+        float x[kBatch][EPL];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const float *q = rec + (size_t)min(i0 + u, m.parts - 1) * tree_record_floats(D);
+            ml[u] = *(const float2 *)q;
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) x[u][i] = q[4 + lane + 64 * i];
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const float weight = i0 + u < m.parts ? __builtin_amdgcn_exp2f(ml[u].x - mx) : 0.0f;
+            l = fmaf(ml[u].y, weight, l);
+#pragma unroll
+            for (int i = 0; i < EPL; ++i) o[i] = fmaf(x[u][i], weight, o[i]);
+        }
+    }
+    const bool gated = (c.flags & SAFETYRAISE_MI355X_GATED) != 0;
+    const bool bf16_in = (c.flags & SAFETYRAISE_MI355X_INPUT_BF16) != 0;
+    const size_t out_row = (size_t)(m.row0 + sr) * c.heads + head;
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+        float y = o[i] * inv;
+        if (gated) y *= ref_sigmoid(load_act(c.q, out_row * 2 * D + D + lane + 64 * i, bf16_in));
+        store_out(c, out_row * D + lane + 64 * i, y);
+    }
+}
+
+template <int D, int VG, bool kF32>
+hipError_t launch_attn(hipStream_t stream, const TreeCommon &c, uint32_t blocks) {
+    using T = TreeShape<D, VG, kF32>;
+    static_assert(T::kLds <= 160 * 1024, "LDS");
+    static const hipError_t configured =
+        hipFuncSetAttribute((const void *)tree_attn_kernel<D, VG, kF32>,
+                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)T::kLds);
+    if (configured != hipSuccess) return configured;
+    SR_LAUNCH("tree_attn_kernel", (tree_attn_kernel<D, VG, kF32>), dim3(blocks), dim3(T::kThreads),
+              T::kLds, stream, c);
+    return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_width(hipStream_t stream, const TreeCommon &c, uint32_t blocks, uint32_t rows,
+                        uint32_t vector_waves) {
+    const bool f32 = (c.flags & SAFETYRAISE_MI355X_OUTPUT_BF16) == 0;
+    hipError_t e = hipErrorInvalidValue;
+    if (vector_waves == 1) {
+        e = f32 ? launch_attn<D, 1, true>(stream, c, blocks) : launch_attn<D, 1, false>(stream, c, blocks);
+    } else if (vector_waves == 2) {
+        e = f32 ? launch_attn<D, 2, true>(stream, c, blocks) : launch_attn<D, 2, false>(stream, c, blocks);
+    } else if constexpr (tree_vector_waves(D) == 4) {
+        e = f32 ? launch_attn<D, 4, true>(stream, c, blocks) : launch_attn<D, 4, false>(stream, c, blocks);
+    }
+    if (e != hipSuccess || c.records == nullptr) return e;
+    SR_LAUNCH("tree_combine_kernel", tree_combine_kernel<D>, dim3((rows * c.heads + 3) / 4), dim3(256),
+              0, stream, c, rows);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+TreeScratch tree_scratch(const TreeLaunch &a, const SeqMeta *seqs, int nseq, uint64_t call_rows,
+                         int num_cus) {
+    TreeScratch t;
+    const size_t group = a.heads / a.kv_heads;
+    uint64_t rows = 0, tiles = 0;
+    for (int i = 0; i < nseq; ++i) {
+        rows += seqs[i].rows;
+        tiles += a.kv_heads * ((seqs[i].rows * group + 31) / 32);
+    }
+    t.mask_bytes = call_rows * sizeof(uint4);
+    if (generic_head_dim(a.head_dim)) {
+        t.q_bytes = rows * a.heads * a.head_dim * sizeof(float);
+        return t;
+    }
+    const size_t parts = (a.flags & SAFETYRAISE_MI355X_OUTPUT_BF16) ? 2 : 3;
+    t.q_bytes = tiles * 32 * a.head_dim * 2 * parts;
+    t.record_bytes = tree_plan(a.heads, a.kv_heads, a.head_dim, a.pool->page_tokens, num_cus, seqs, nseq).record_bytes;
+    return t;
+}
+
+hipError_t launch_tree_attn(hipStream_t stream, const TreeLaunch &a, const SeqMeta *seqs, int nseq,
+                            const uint8_t *parents, int num_cus) {
+    PrepParams p{};
+    TreeCommon &c = p.c;
+    const auto *pool = a.pool;
+    const bool generic = generic_head_dim(a.head_dim);
+    const uint32_t D = a.head_dim;
+    uint32_t rows = 0;
+    for (int i = 0; i < nseq; ++i) rows += seqs[i].rows;
+    if (nseq <= 0 || nseq > (int)kTreeSeqs || rows > kTreeRows || a.tbl_n > kInlineTable ||
+        a.rotary_dim > D || D > kGenericMaxHeadDim) {
+        return hipErrorInvalidValue;
+    }
+    c.k_pages = pool->k_pages;
+    c.v_pages = pool->v_pages;
+    c.page_table = pool->d_page_table;
+    c.q = a.q;
+    c.q_ops = a.q_ops;
+    c.masks = (uint4 *)a.masks;
+    c.out = a.out;
+    c.err_word = a.err_word;
+    c.num_pages = pool->num_pages;
+    c.pages_per_seq = pool->pages_per_seq;
+    c.log2_page = (uint32_t)__builtin_ctz(pool->page_tokens);
+    c.flags = a.flags;
+    c.heads = a.heads;
+    c.kv_heads = a.kv_heads;
+    c.head_dim = D;
+    c.nseq = (uint32_t)nseq;
+    TreePlan plan{};
+    if (!generic) {
+        plan = tree_plan(a.heads, a.kv_heads, D, pool->page_tokens, num_cus, seqs, nseq);
+        c.part_keys = plan.part_keys;
+        c.records = plan.direct ? nullptr : a.records;
+        if (!plan.direct && a.records == nullptr) return hipErrorInvalidValue;
+    }
+    uint32_t blocks = 0, tiles = 0, records = 0;
+    const uint32_t group = a.heads / a.kv_heads;
+    for (int i = 0; i < nseq; ++i) {
+        TreeMeta &m = c.meta[i];
+        m.slot = seqs[i].slot;
+        m.ctx = seqs[i].ctx;
+        m.rows = seqs[i].rows;
+        m.row0 = seqs[i].row0;
+        m.tile0 = tiles;
+        tiles += a.kv_heads * ((m.rows * group + 31) / 32);
+        if (generic) continue;
+        m.block0 = blocks;
+        m.record0 = records;
+        m.parts = (m.ctx + m.rows + plan.part_keys - 1) / plan.part_keys;
+        const uint32_t per = plan.vector_waves * kTreeVectors;
+        blocks += m.parts * a.kv_heads * ((m.rows * group + per - 1) / per);
+        records += m.parts * m.rows * a.heads;
+    }
+    p.k = a.k;
+    p.v = a.v;
+    // without QK-norm the weights are not read
+    p.q_norm = a.q_norm;
+    p.k_norm = a.k_norm;
+    p.positions = a.positions;
+    p.rotary_dim = a.rotary_dim;
+    for (int i = 0; i < 3; ++i) p.mrope[i] = a.mrope[i];
+    p.eps = a.eps;
+    p.qscale = kLog2e / sqrtf((float)D);
+    p.rows = rows;
+    p.parts = generic ? 0 : (a.flags & SAFETYRAISE_MI355X_OUTPUT_BF16) ? 2 : 3;
+    p.tbl_n = a.tbl_n;
+    for (uint32_t i = 0; i < a.tbl_n; ++i) {
+        p.tbl_idx[i] = a.tbl_idx[i];
+        p.tbl_val[i] = a.tbl_val[i];
+    }
+    for (uint32_t i = 0; i < a.rotary_dim / 2; ++i) p.denom[i] = a.rope_denom[i];
+    for (uint32_t i = 0; i < rows; ++i) p.parent[i] = parents[i];
+    const uint32_t groups = (a.kv_heads + a.heads + kPrepHeads - 1) / kPrepHeads;
+    const dim3 grid((rows * groups + 3) / 4);
+    const size_t prep_lds = (size_t)4 * kPrepHeads * D * sizeof(float);
+    if (D <= 64) SR_LAUNCH("tree_prep_kernel", tree_prep_kernel<1>, grid, dim3(256), prep_lds, stream, p);
+    else if (D <= 128) SR_LAUNCH("tree_prep_kernel", tree_prep_kernel<2>, grid, dim3(256), prep_lds, stream, p);
+    else if (D <= 256) SR_LAUNCH("tree_prep_kernel", tree_prep_kernel<4>, grid, dim3(256), prep_lds, stream, p);
+    else SR_LAUNCH("tree_prep_kernel", tree_prep_kernel<8>, grid, dim3(256), prep_lds, stream, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    switch (D) {
+        case 64: return launch_width<64>(stream, c, blocks, rows, plan.vector_waves);
+        case 128: return launch_width<128>(stream, c, blocks, rows, plan.vector_waves);
+        case 256: return launch_width<256>(stream, c, blocks, rows, plan.vector_waves);
+        default: break;
+    }
+    SR_LAUNCH("tree_generic_kernel", tree_generic_kernel, dim3(a.heads, rows), dim3(64),
+              (D + 64) * sizeof(float), stream, c);
+    return hipGetLastError();
+}
+
+}  // namespace sr

@@ -55,6 +55,10 @@ NORM_OFFSET = 0x10
 GATED = 0x20
 MROPE_INTERLEAVED = 0x40
 KEEP_ROWS = 0x80
+OUTPUT_BF16 = 0x100
+
+MAX_TREE_ROWS = 128
+MAX_GDN_TREE_ROWS = 64
 
 V1_SYMBOLS = (
     "safetyraise_kernel_abi_version",
@@ -91,6 +95,12 @@ EXTENSION_SYMBOLS = (
     "safetyraise_kernel_gdn_write",
     "safetyraise_kernel_gdn_forward",
     "safetyraise_kernel_gdn_rollback",
+    "safetyraise_kernel_attention_tree_forward",
+    "safetyraise_kernel_gdn_tree_forward",
+    "safetyraise_kernel_gdn_tree_commit",
+    "safetyraise_kernel_gdn_view",
+    "safetyraise_kernel_kv_compact",
+    "safetyraise_kernel_kv_gather",
     "safetyraise_kernel_linear_device",
     "safetyraise_kernel_timing_enable",
     "safetyraise_kernel_timing_read",
@@ -185,6 +195,50 @@ class GdnArgs(C.Structure):
     ]
 
 
+class AttentionTreeArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("reserved", C.c_uint32),
+        ("attention", AttentionArgs),
+        ("parents", C.POINTER(C.c_int32)),
+    ]
+
+
+class GdnTreeArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("reserved", C.c_uint32),
+        ("gdn", GdnArgs),
+        ("parents", C.POINTER(C.c_int32)),
+    ]
+
+
+class GdnCommit(C.Structure):
+    _fields_ = [("state", C.c_void_p), ("sequence", C.c_uint32), ("row", C.c_int32)]
+
+
+class KvKeep(C.Structure):
+    _fields_ = [
+        ("kv", C.c_void_p),
+        ("source", C.c_uint32),
+        ("target", C.c_uint32),
+        ("start", C.c_uint64),
+        ("count", C.c_uint64),
+        ("tokens", C.POINTER(C.c_uint32)),
+    ]
+
+
+class KvRows(C.Structure):
+    _fields_ = [
+        ("kv", C.c_void_p),
+        ("sequence", C.c_uint32),
+        ("reserved", C.c_uint32),
+        ("start", C.c_uint64),
+        ("count", C.c_uint64),
+        ("tokens", C.POINTER(C.c_uint32)),
+    ]
+
+
 class PluginError(RuntimeError):
     """A non-zero plugin status, formatted like the engine's WeightError."""
 
@@ -230,6 +284,12 @@ def _declare(lib: C.CDLL) -> None:
         "safetyraise_kernel_gdn_write": (i32, [vp, vp, u32, vp, vp]),
         "safetyraise_kernel_gdn_forward": (i32, [vp, C.POINTER(GdnArgs)]),
         "safetyraise_kernel_gdn_rollback": (i32, [vp, vp, u32, u32, u32]),
+        "safetyraise_kernel_attention_tree_forward": (i32, [vp, C.POINTER(AttentionTreeArgs)]),
+        "safetyraise_kernel_gdn_tree_forward": (i32, [vp, C.POINTER(GdnTreeArgs)]),
+        "safetyraise_kernel_gdn_tree_commit": (i32, [vp, C.POINTER(GdnCommit), u32, u32]),
+        "safetyraise_kernel_gdn_view": (i32, [vp, vp, u32, C.POINTER(vp), C.POINTER(vp)]),
+        "safetyraise_kernel_kv_compact": (i32, [vp, C.POINTER(KvKeep), u32, u32]),
+        "safetyraise_kernel_kv_gather": (i32, [vp, C.POINTER(KvRows), u32, vp, vp, u32]),
         "safetyraise_kernel_linear_device": (i32, [vp, vp, vp, u64, u64, vp, u64, u64]),
         "safetyraise_kernel_timing_enable": (i32, [vp, u32]),
         "safetyraise_kernel_timing_read": (i32, [vp, u32, C.POINTER(C.c_char_p), pu64,
@@ -501,6 +561,17 @@ def attention_forward(backend: NativeBackend, kv: KvCache, seq_ids: Sequence[int
                       norm_offset: bool = False, mrope_section=(0, 0, 0),
                       mrope_interleaved: bool = True, asynchronous: bool = False) -> None:
     """Attention::forward row loop (src/model/native.rs:615-645) for a batch."""
+    args = _attention_args(kv, seq_ids, seq_rows, q, k, v, positions, out, heads, kv_heads, head_dim,
+                           rotary_dim, rope_theta, eps, q_norm, k_norm, gated, norm_offset,
+                           mrope_section, mrope_interleaved, asynchronous)
+    backend.check(backend.lib.safetyraise_kernel_attention_forward(backend.context,
+                                                                    C.byref(args)),
+                  "attention_forward")
+
+
+def _attention_args(kv, seq_ids, seq_rows, q, k, v, positions, out, heads, kv_heads, head_dim,
+                    rotary_dim, rope_theta, eps, q_norm, k_norm, gated, norm_offset, mrope_section,
+                    mrope_interleaved, asynchronous) -> AttentionArgs:
     flags = 0
     if _is_device(q):
         flags |= DEVICE_POINTERS
@@ -534,9 +605,79 @@ def attention_forward(backend: NativeBackend, kv: KvCache, seq_ids: Sequence[int
     args.positions = _ptr(positions)
     args.out = _ptr(out)
     args.kv = kv.handle
-    backend.check(backend.lib.safetyraise_kernel_attention_forward(backend.context,
-                                                                    C.byref(args)),
-                  "attention_forward")
+    return args
+
+
+def _tree_parents(parents: Sequence[int], seq_rows: Sequence[int]):
+    if len(parents) != sum(seq_rows):
+        raise ValueError("parents has one entry per row of the call")
+    return (C.c_int32 * max(1, len(parents)))(*parents)
+
+
+def attention_tree_forward(backend: NativeBackend, kv: KvCache, seq_ids: Sequence[int],
+                           seq_rows: Sequence[int], parents: Sequence[int], q, k, v, positions, out,
+                           *, heads: int, kv_heads: int, head_dim: int, rotary_dim: int,
+                           rope_theta: float, eps: float = 1e-6, q_norm=None, k_norm=None,
+                           gated: bool = False, norm_offset: bool = False, mrope_section=(0, 0, 0),
+                           mrope_interleaved: bool = True, asynchronous: bool = False) -> None:
+    """attention_forward for trees of drafts: row r sees the context, its ancestors
+    (parents[r]: a row of the same sequence, -1 behind the context) and itself.
+    out is float32, or bfloat16 (a torch tensor)."""
+    args = AttentionTreeArgs()
+    args.struct_size = C.sizeof(AttentionTreeArgs)
+    args.attention = _attention_args(kv, seq_ids, seq_rows, q, k, v, positions, out, heads, kv_heads,
+                                     head_dim, rotary_dim, rope_theta, eps, q_norm, k_norm, gated,
+                                     norm_offset, mrope_section, mrope_interleaved, asynchronous)
+    if str(getattr(out, "dtype", "")).endswith("bfloat16"):
+        args.attention.flags |= OUTPUT_BF16
+    args.parents = _tree_parents(parents, seq_rows)
+    backend.check(backend.lib.safetyraise_kernel_attention_tree_forward(backend.context,
+                                                                         C.byref(args)),
+                  "attention_tree_forward")
+
+
+def kv_compact(backend: NativeBackend, keeps, asynchronous: bool = False) -> None:
+    """Keeps chosen tokens of sequences.  keeps: (kv, source, target, start, tokens)
+    per entry: the first `start` tokens and start + tokens[i] (ascending) become
+    target's contents (target == source: in place)."""
+    entries = (KvKeep * max(1, len(keeps)))()
+    lists = []
+    for e, (kv, source, target, start, tokens) in zip(entries, keeps):
+        lists.append((C.c_uint32 * max(1, len(tokens)))(*tokens))
+        e.kv, e.source, e.target, e.start, e.count = kv.handle, source, target, start, len(tokens)
+        e.tokens = lists[-1]
+    backend.check(backend.lib.safetyraise_kernel_kv_compact(
+        backend.context, entries, len(keeps), ASYNC if asynchronous else 0), "kv_compact")
+
+
+def kv_gather(backend: NativeBackend, reads, keys, values, asynchronous: bool = False) -> None:
+    """Copies tokens of sequences into keys and values [tokens][kv_heads * head_dim]
+    (float32, or bfloat16 torch tensors).  reads: (kv, sequence, start, tokens) per
+    entry, tokens a list counted from start, or their number."""
+    entries = (KvRows * max(1, len(reads)))()
+    lists = []
+    for e, (kv, sequence, start, tokens) in zip(entries, reads):
+        e.kv, e.sequence, e.start = kv.handle, sequence, start
+        if isinstance(tokens, int):
+            e.count = tokens
+        else:
+            lists.append((C.c_uint32 * max(1, len(tokens)))(*tokens))
+            e.count, e.tokens = len(tokens), lists[-1]
+    flags = 0
+    if _is_device(keys):
+        flags |= DEVICE_POINTERS | (ASYNC if asynchronous else 0)
+    if str(getattr(keys, "dtype", "")).endswith("bfloat16"):
+        flags |= OUTPUT_BF16
+    backend.check(backend.lib.safetyraise_kernel_kv_gather(
+        backend.context, entries, len(reads), _ptr(keys), _ptr(values), flags), "kv_gather")
+
+
+class _DeviceArray:
+    """f32 device memory for torch.as_tensor."""
+
+    def __init__(self, pointer: int, shape):
+        self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": "<f4", "version": 2,
+                                         "data": (pointer, False), "strides": None}
 
 
 class GdnState:
@@ -584,6 +725,18 @@ class GdnState:
         h = np.ascontiguousarray(history, dtype=np.float32)
         self._call("write", seq, m.ctypes.data, h.ctypes.data)
 
+    def view(self, seq: int):
+        """The current state [Hv][Dv][Dk] and history [C][K-1] as torch tensors on
+        the pool's own memory, valid until the sequence changes."""
+        import torch
+
+        matrix, history = C.c_void_p(), C.c_void_p()
+        self._call("view", seq, C.byref(matrix), C.byref(history))
+        shapes = ((self.value_heads, self.value_dim, self.key_dim),
+                  (self.channels, self.conv_kernel - 1))
+        return tuple(torch.as_tensor(_DeviceArray(p.value, shape), device="cuda")
+                     for p, shape in zip((matrix, history), shapes))
+
     def rollback(self, seq: int, rows: int, asynchronous: bool = False) -> None:
         """State and history after the first `rows` rows of the last KEEP_ROWS call."""
         self._call("rollback", seq, rows, ASYNC if asynchronous else 0)
@@ -599,7 +752,16 @@ def gdn_forward(backend: NativeBackend, state: GdnState, seq_ids: Sequence[int],
                 *, eps: float = 1e-6, asynchronous: bool = False, keep_rows: bool = False) -> None:
     """Gdn::forward row loop (src/model/native.rs:720-742) for a batch; keep_rows
     records every row so that GdnState.rollback can return to any of them."""
-    flags = KEEP_ROWS if keep_rows else 0
+    args = _gdn_args(state, seq_ids, seq_rows, qkv, z, a, b, a_log, dt_bias, conv_weight, norm, out,
+                     eps, asynchronous)
+    args.flags |= KEEP_ROWS if keep_rows else 0
+    backend.check(backend.lib.safetyraise_kernel_gdn_forward(backend.context, C.byref(args)),
+                  "gdn_forward")
+
+
+def _gdn_args(state, seq_ids, seq_rows, qkv, z, a, b, a_log, dt_bias, conv_weight, norm, out, eps,
+              asynchronous) -> GdnArgs:
+    flags = 0
     if _is_device(qkv):
         flags |= DEVICE_POINTERS
         if asynchronous:
@@ -619,5 +781,29 @@ def gdn_forward(backend: NativeBackend, state: GdnState, seq_ids: Sequence[int],
     args.conv_weight, args.norm = _ptr(conv_weight), _ptr(norm)
     args.out = _ptr(out)
     args.state = state.handle
-    backend.check(backend.lib.safetyraise_kernel_gdn_forward(backend.context, C.byref(args)),
-                  "gdn_forward")
+    return args
+
+
+def gdn_tree_forward(backend: NativeBackend, state: GdnState, seq_ids: Sequence[int],
+                     seq_rows: Sequence[int], parents: Sequence[int], qkv, z, a, b, a_log, dt_bias,
+                     conv_weight, norm, out, *, eps: float = 1e-6,
+                     asynchronous: bool = False) -> None:
+    """gdn_forward for trees of drafts (parents as in attention_tree_forward): each
+    row continues from its parent; the states stay until gdn_tree_commit."""
+    args = GdnTreeArgs()
+    args.struct_size = C.sizeof(GdnTreeArgs)
+    args.gdn = _gdn_args(state, seq_ids, seq_rows, qkv, z, a, b, a_log, dt_bias, conv_weight, norm,
+                         out, eps, asynchronous)
+    args.parents = _tree_parents(parents, seq_rows)
+    backend.check(backend.lib.safetyraise_kernel_gdn_tree_forward(backend.context, C.byref(args)),
+                  "gdn_tree_forward")
+
+
+def gdn_tree_commit(backend: NativeBackend, commits, asynchronous: bool = False) -> None:
+    """commits: (state, sequence, row) per entry; the state and history after that
+    row of the sequence's last gdn_tree_forward (-1: before it)."""
+    entries = (GdnCommit * max(1, len(commits)))()
+    for e, (state, sequence, row) in zip(entries, commits):
+        e.state, e.sequence, e.row = state.handle, sequence, row
+    backend.check(backend.lib.safetyraise_kernel_gdn_tree_commit(
+        backend.context, entries, len(commits), ASYNC if asynchronous else 0), "gdn_tree_commit")
