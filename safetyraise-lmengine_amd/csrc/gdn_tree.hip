@@ -202,6 +202,325 @@ __global__ void __launch_bounds__(256) gdn_tree_generic_kernel(const GdnTreePara
     }
 }
 
+// ---------------------------------------------------------------------------
+// Dk = Dv = 128: one workgroup of 8 waves per (value head, sequence), everything
+// between the inputs and the outputs in LDS and registers.
+//
+// Wave w owns state rows 16 w .. 16 w + 15 (32 registers, requested first) and
+// the same columns of every [row][Dv] matrix.  With X = diag(norms) applied
+// where a product is used:
+//   1. raw conv inputs to LDS behind the history; decays, ancestors, conv taps
+//      (one wave, pointer doubling over the parents)
+//   2. conv + silu in place, last row first (a row reads rows before it)
+//   3. norms of q and k
+//   4. K S0^T and Q S0^T per wave; K K^T and Q K^T blocks over the waves, masked
+//      and decayed:  A[t][j] = -b_t e^{g_t - g_j} (k^_t . k^_j),  j above t
+//                    P[t][j] = e^{g_t - g_j} (q^_t . k^_j),       j above or t
+//   5. T = (I - A_bb)^-1 of each 16-row block
+//   6. block by block  D_b = T_b (b_t (V - e^{g_t} K^ S0^T) + sum_{c<b} A_bc D_c),
+//      O_b = e^{g_t} Q^ S0^T + sum_{c<=b} P_bc D_c
+//   7. RMSNorm and gate, a row per wave.
+// All products are v_mfma_f32_16x16x4_f32 with both operands 4 consecutive k per
+// lane; an accumulator (rows 4 g + i of lane group g) is the next product's B
+// operand as it is.
+// RT: 16-row tiles of the longest tree.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kW = 128;         // Dk and Dv
+constexpr uint32_t kPitch = kW + 4;  // floats per LDS row (16 rows of 16 bytes meet no bank twice)
+constexpr uint32_t kHist = 7;        // history rows in front of the tree's
+
+template <int RT>
+struct HeadShape {
+    static constexpr uint32_t kRows = 16 * RT;
+    static constexpr uint32_t kPart = (kHist + kRows) * kPitch;  // floats of q, k or v
+    static constexpr uint32_t kPair = kRows + 4;                 // pitch of A and P
+    static constexpr size_t kLds = (3 * kPart + 2 * kRows * kPair) * sizeof(float);
+};
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// acc += A . B over 16 k: element i of both operands per instruction
+__device__ __forceinline__ f32x4 mma16(const f32x4 &a, const f32x4 &b, f32x4 acc) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc, 0, 0, 0);
+    return acc;
+}
+
+// x * sigmoid(x) with the hardware exp2 and reciprocal
+__device__ __forceinline__ float silu_fast(float x) {
+    return x * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * x));
+}
+
+template <int RT>
+__global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams p) {
+    using T = HeadShape<RT>;
+    constexpr uint32_t kPair = T::kPair;
+    extern __shared__ __align__(16) float lds[];
+    __shared__ double g_s[kRowsMax];
+    __shared__ uint64_t anc_s[kRowsMax];
+    __shared__ float beta_s[kRowsMax], decay_s[kRowsMax], qn_s[kRowsMax], kn_s[kRowsMax];
+    __shared__ int tap_s[kRowsMax][8];
+    float *xq = lds, *xk = lds + T::kPart, *xv = lds + 2 * T::kPart;
+    float *As = lds + 3 * T::kPart, *Ps = As + T::kRows * kPair;
+
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = (uint32_t)wave_index();
+    const uint32_t h = blockIdx.x;
+    const TreeMeta m = p.meta[blockIdx.y];
+    const uint32_t R = m.rows, rt = (R + 15) / 16;
+    const uint32_t groups = p.value_heads / p.key_heads, kh = h / groups;
+    const bool first_of_key = h % groups == 0;
+    const bool bf16 = p.bf16_in != 0;
+    const uint32_t K = p.conv_k, K1 = K - 1;
+    const uint32_t l16 = lane & 15, g4 = lane >> 4;
+    float *rec = p.records + (size_t)m.slot * p.keep_rows * p.rec_stride;
+
+    // the wave's state rows: row 16 w + l16, dims 16 s + 4 g4 .. + 3
+    f32x4 S[8];
+    {
+        const float *src = p.state + (((size_t)m.state_in * p.value_heads + h) * kW + 16 * wave + l16) * kW + 4 * g4;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) S[s] = __builtin_nontemporal_load((const f32x4 *)(src + 16 * s));
+    }
+    // 1.
+    const uint32_t part = wave >> 1, c = tid & 127;  // q, k, v; waves 6 and 7 have no channel
+    const uint32_t ch = part == 0 ? kh * kW + c
+                      : part == 1 ? (p.key_heads + kh) * kW + c
+                                  : 2 * p.key_heads * kW + h * kW + c;
+    float *X = lds + part * T::kPart + c;
+    float w[8];
+    if (part < 3) {
+        const float *hist = p.history + (((size_t)m.parity * p.max_slots + m.slot) * p.channels + ch) * K1;
+        float x[T::kRows], old[kHist];
+#pragma unroll
+        for (uint32_t i = 0; i < T::kRows; ++i) {
+            x[i] = load_act_nb(p.qkv, (size_t)(m.row0 + min(i, R - 1)) * p.channels + ch, bf16);
+        }
+        // (the history holds at least one value, also for K = 1)
+#pragma unroll
+        for (uint32_t j = 0; j < kHist; ++j) old[j] = hist[j < K1 ? j : 0];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) w[j] = p.conv_w[(size_t)ch * K + (j < K ? j : 0)];
+#pragma unroll
+        for (uint32_t j = 0; j < kHist; ++j) {
+            if (j < K1) X[(kHist - K1 + j) * kPitch] = old[j];
+        }
+        const bool owns = part == 2 || first_of_key;
+#pragma unroll
+        for (uint32_t i = 0; i < T::kRows; ++i) {
+            X[(kHist + i) * kPitch] = i < R ? x[i] : 0.0f;
+            if (owns && i < R) rec[(size_t)i * p.rec_stride + rec_raw(p) + ch] = x[i];
+        }
+    } else if (wave == 6) {
+        const uint32_t r = min(lane, R - 1);
+        const float av = load_act(p.a, (size_t)(m.row0 + r) * p.value_heads + h, bf16);
+        const float bv = load_act(p.b, (size_t)(m.row0 + r) * p.value_heads + h, bf16);
+        const int up = (int)p.parent[m.row0 - p.meta[0].row0 + r] - 1;
+        const float log_a = -expf(p.a_log[h]) * softplus_ref(av + p.dt_bias[h]);
+        // the path's set and sum up to, not with, `next`: doubling
+        int next = up;
+        uint32_t lo = r < 32 ? 1u << r : 0u, hi = r < 32 ? 0u : 1u << (r - 32);
+        double sum = (double)log_a;
+#pragma unroll
+        for (int step = 0; step < 6; ++step) {
+            const int at = next < 0 ? (int)lane : next;
+            const uint32_t l2 = __shfl(lo, at), h2 = __shfl(hi, at);
+            const double s2 = __shfl(sum, at);
+            const int n2 = __shfl(next, at);
+            if (next >= 0) {
+                lo |= l2;
+                hi |= h2;
+                sum += s2;
+                next = n2;
+            }
+        }
+        int at = (int)r, back = 0;
+        for (uint32_t j = 0; j < K; ++j) {
+            const int u = __shfl(up, at < 0 ? 0 : at);
+            if (lane < R) tap_s[lane][j] = at >= 0 ? (int)kHist + at : (int)kHist - 1 - back;
+            back += at < 0 ? 1 : 0;
+            at = at < 0 ? -1 : u;
+        }
+        if (lane < R) {
+            g_s[lane] = sum;
+            anc_s[lane] = ((uint64_t)hi << 32) | lo;
+            beta_s[lane] = ref_sigmoid(bv);
+            decay_s[lane] = (float)exp(sum);
+            rec[(size_t)lane * p.rec_stride + h] = expf(log_a);
+        } else {
+            // rows of the last tile past the tree
+            g_s[lane] = 0.0;
+            anc_s[lane] = 0;
+            beta_s[lane] = decay_s[lane] = qn_s[lane] = kn_s[lane] = 0.0f;
+        }
+    }
+    __syncthreads();
+    // 2. oldest tap first, as the reference sums them (math.rs:175-185)
+    if (part < 3) {
+        for (int t0 = (int)R - 1; t0 >= 0; t0 -= 4) {
+            float acc[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = max(t0 - i, 0);
+                acc[i] = 0.0f;
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) {
+                    if (j < K) acc[i] = fmaf(X[tap_s[t][K1 - j] * kPitch], w[j], acc[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (t0 - i >= 0) X[(kHist + t0 - i) * kPitch] = silu_fast(acc[i]);
+            }
+        }
+    }
+    __syncthreads();
+    // 3.
+    for (uint32_t t = wave; t < 2 * R; t += 8) {
+        const float *y = ((t & 1) ? xk : xq) + (kHist + (t >> 1)) * kPitch;
+        const float y0 = y[lane], y1 = y[lane + 64];
+        const float ss = sum64(fmaf(y1, y1, y0 * y0));
+        const float inv = 1.0f / sqrtf(ss + 1e-6f);
+        if (lane == 0) ((t & 1) ? kn_s : qn_s)[t >> 1] = inv;
+        if ((t & 1) && first_of_key) {
+            float *key = rec + (size_t)(t >> 1) * p.rec_stride + rec_key(p) + kh * kW;
+            key[lane] = y0 * inv;
+            key[lane + 64] = y1 * inv;
+        }
+    }
+    // 4.
+    f32x4 kS[RT], qS[RT];
+#pragma unroll
+    for (int b = 0; b < RT; ++b) kS[b] = qS[b] = f32x4{};
+#pragma unroll
+    for (int b = 0; b < RT; ++b) {
+        if ((uint32_t)b >= rt) break;
+        const float *kr = xk + (kHist + 16 * b + l16) * kPitch + 4 * g4;
+        const float *qr = xq + (kHist + 16 * b + l16) * kPitch + 4 * g4;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            kS[b] = mma16(*(const f32x4 *)(kr + 16 * s), S[s], kS[b]);
+            qS[b] = mma16(*(const f32x4 *)(qr + 16 * s), S[s], qS[b]);
+        }
+    }
+    __syncthreads();
+    {
+        // blocks (bt, bj), bj <= bt, of K K^T, then of Q K^T
+        const uint32_t blocks = rt * (rt + 1);
+        for (uint32_t i = wave; i < blocks; i += 8) {
+            const bool is_q = i >= blocks / 2;
+            uint32_t bj = is_q ? i - blocks / 2 : i, bt = 0;
+            while (bj > bt) bj -= ++bt;
+            const float *ar = (is_q ? xq : xk) + (kHist + 16 * bt + l16) * kPitch + 4 * g4;
+            const float *br = xk + (kHist + 16 * bj + l16) * kPitch + 4 * g4;
+            f32x4 acc[2] = {f32x4{}, f32x4{}};
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                acc[s & 1] = mma16(*(const f32x4 *)(ar + 16 * s), *(const f32x4 *)(br + 16 * s), acc[s & 1]);
+            }
+            const uint32_t j = 16 * bj + l16;
+            const double gj = g_s[j];
+            const float kj = kn_s[j];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t t = 16 * bt + 4 * g4 + e;
+                const bool sees = (anc_s[t] >> j) & 1;
+                const float ratio = __builtin_amdgcn_exp2f((float)(g_s[t] - gj) * kLog2e);
+                const float dot = (acc[0][e] + acc[1][e]) * kj;
+                if (is_q) Ps[t * kPair + j] = sees ? dot * qn_s[t] * ratio : 0.0f;
+                else As[t * kPair + j] = sees && t != j ? -dot * kn_s[t] * ratio * beta_s[t] : 0.0f;
+            }
+        }
+    }
+    // (the rows' z, for step 7)
+    const size_t width = (size_t)p.value_heads * kW;
+    float z0[2 * RT], z1[2 * RT];
+#pragma unroll
+    for (int i = 0; i < 2 * RT; ++i) {
+        const size_t at = (size_t)(m.row0 + min(wave + 8 * i, R - 1)) * width + h * kW + lane;
+        z0[i] = load_act_nb(p.z, at, bf16);
+        z1[i] = load_act_nb(p.z, at + 64, bf16);
+    }
+    __syncthreads();
+    // 5. column l16 of the inverse per lane
+    if (wave < rt) {
+        float *Ab = As + 16 * wave * kPair + 16 * wave;
+        float x[16];
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            float acc = (uint32_t)t == l16 ? 1.0f : 0.0f;
+#pragma unroll
+            for (int i = 0; i < t; ++i) acc = fmaf(Ab[t * kPair + i], x[i], acc);
+            x[t] = acc;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (lane < 16) {
+#pragma unroll
+            for (int t = 0; t < 16; ++t) Ab[t * kPair + lane] = x[t];
+        }
+    }
+    __syncthreads();
+    // 6.
+    const float qscale = 0.08838834764831845f;  // 1 / sqrt(128)
+    f32x4 D[RT];
+#pragma unroll
+    for (int b = 0; b < RT; ++b) {
+        if ((uint32_t)b >= rt) break;
+        float *vr = xv + (kHist + 16 * b + 4 * g4) * kPitch + 16 * wave + l16;
+        f32x4 rhs, o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t t = 16 * b + 4 * g4 + e;
+            rhs[e] = beta_s[t] * (vr[e * kPitch] - decay_s[t] * kn_s[t] * kS[b][e]);
+            o[e] = decay_s[t] * qn_s[t] * qS[b][e];
+        }
+        const float *Ar = As + (16 * b + l16) * kPair + 4 * g4;
+        const float *Pr = Ps + (16 * b + l16) * kPair + 4 * g4;
+#pragma unroll
+        for (int cc = 0; cc < b; ++cc) {
+            rhs = mma16(*(const f32x4 *)(Ar + 16 * cc), D[cc], rhs);
+            o = mma16(*(const f32x4 *)(Pr + 16 * cc), D[cc], o);
+        }
+        D[b] = mma16(*(const f32x4 *)(Ar + 16 * b), rhs, f32x4{});
+        o = mma16(*(const f32x4 *)(Pr + 16 * b), D[b], o);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t t = 16 * b + 4 * g4 + e;
+            vr[e * kPitch] = o[e] * qscale;
+            if (t < R) rec[(size_t)t * p.rec_stride + rec_delta(p) + h * kW + 16 * wave + l16] = D[b][e];
+        }
+    }
+    __syncthreads();
+    // 7. RMSNorm without offset, then * silu(z) (native.rs:737-740)
+    const float n0 = p.norm[lane], n1 = p.norm[lane + 64];
+#pragma unroll
+    for (int i = 0; i < 2 * RT; ++i) {
+        const uint32_t t = wave + 8 * i;
+        if (t >= R) break;
+        const float *o = xv + (kHist + t) * kPitch;
+        const float o0 = o[lane], o1 = o[lane + 64];
+        const float variance = sum64(fmaf(o1, o1, o0 * o0)) / (float)kW;
+        if (!isfinite(variance) && lane == 0) atomicOr(p.err_word, kErrNonFiniteVariance);
+        const float inv = 1.0f / sqrtf(variance + p.eps);
+        float *dst = p.out + (size_t)(m.row0 + t) * width + h * kW;
+        dst[lane] = o0 * inv * n0 * silu_fast(z0[i]);
+        dst[lane + 64] = o1 * inv * n1 * silu_fast(z1[i]);
+    }
+}
+
+template <int RT>
+hipError_t launch_head(hipStream_t stream, const GdnTreeParams &p) {
+    using T = HeadShape<RT>;
+    static_assert(T::kLds + 8192 <= 160 * 1024, "LDS");
+    static const hipError_t configured =
+        hipFuncSetAttribute((const void *)gdn_tree_head_kernel<RT>,
+                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)T::kLds);
+    if (configured != hipSuccess) return configured;
+    SR_LAUNCH("gdn_tree_head_kernel", gdn_tree_head_kernel<RT>, dim3(p.value_heads, p.nseq), dim3(512),
+              T::kLds, stream, p);
+    return hipGetLastError();
+}
+
 struct CommitParams {
     const GdnCommitEntry *entries;  // nullptr: in the arguments
     GdnCommitEntry inline_entries[kGdnCommitInline];
@@ -278,6 +597,7 @@ __global__ void __launch_bounds__(256) gdn_tree_commit_kernel(const CommitParams
 }  // namespace
 
 size_t gdn_tree_scratch_bytes(const safetyraise_kernel_gdn_pool *pool, uint32_t rows) {
+    if (pool->key_dim == kW && pool->value_dim == kW) return 0;
     return (size_t)rows * pool->channels * sizeof(float);
 }
 
@@ -317,6 +637,16 @@ hipError_t launch_gdn_tree(hipStream_t stream, const GdnLaunch &g, const GdnSeq 
         p.meta[i] = TreeMeta{seqs[i].slot, seqs[i].rows, seqs[i].row0, seqs[i].parity, seqs[i].state_in};
         for (uint32_t r = 0; r < seqs[i].rows; ++r) p.parent[p.rows + r] = parents[p.rows + r];
         p.rows += seqs[i].rows;
+    }
+    uint32_t most = 0;
+    for (int i = 0; i < nseq; ++i) most = std::max(most, seqs[i].rows);
+    if (p.key_dim == kW && p.value_dim == kW) {
+        switch ((most + 15) / 16) {
+            case 1: return launch_head<1>(stream, p);
+            case 2: return launch_head<2>(stream, p);
+            case 3: return launch_head<3>(stream, p);
+            default: return launch_head<4>(stream, p);
+        }
     }
     SR_LAUNCH("gdn_tree_conv_kernel", gdn_tree_conv_kernel, dim3((p.channels + 255) / 256, p.rows),
               dim3(256), 0, stream, p);
