@@ -16,6 +16,7 @@
 // Records per row (the pool's, see gdn_rollback): a [Hv], d [Hv][Dv], k^ [Hk][Dk],
 // raw conv inputs [C]; gdn_tree_commit_kernel builds the state of a path from them.
 #include <algorithm>
+#include <type_traits>
 
 #include "sr_device.hpp"
 #include "tree_plan.hpp"
@@ -207,12 +208,11 @@ __global__ void __launch_bounds__(256) gdn_tree_generic_kernel(const GdnTreePara
 // between the inputs and the outputs in LDS and registers.
 //
 // Wave w owns state rows 16 w .. 16 w + 15 (32 registers, requested first) and
-// the same columns of every [row][Dv] matrix.  With X = diag(norms) applied
-// where a product is used:
+// the same columns of every [row][Dv] matrix:
 //   1. raw conv inputs to LDS behind the history; decays, ancestors, conv taps
 //      (one wave, pointer doubling over the parents)
 //   2. conv + silu in place, last row first (a row reads rows before it)
-//   3. norms of q and k
+//   3. q and k normalised, as fp16 parts
 //   4. K S0^T and Q S0^T per wave; K K^T and Q K^T blocks over the waves, masked
 //      and decayed:  A[t][j] = -b_t e^{g_t - g_j} (k^_t . k^_j),  j above t
 //                    P[t][j] = e^{g_t - g_j} (q^_t . k^_j),       j above or t
@@ -220,9 +220,8 @@ __global__ void __launch_bounds__(256) gdn_tree_generic_kernel(const GdnTreePara
 //   6. block by block  D_b = T_b (b_t (V - e^{g_t} K^ S0^T) + sum_{c<b} A_bc D_c),
 //      O_b = e^{g_t} Q^ S0^T + sum_{c<=b} P_bc D_c
 //   7. RMSNorm and gate, a row per wave.
-// All products are v_mfma_f32_16x16x4_f32 with both operands 4 consecutive k per
-// lane; an accumulator (rows 4 g + i of lane group g) is the next product's B
-// operand as it is.
+// The products of step 6 are v_mfma_f32_16x16x4_f32 with 4 consecutive k per lane; an
+// accumulator (rows 4 g + i of lane group g) is the next product's B operand as it is.
 // RT: 16-row tiles of the longest tree.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kW = 128;         // Dk and Dv
@@ -238,6 +237,28 @@ struct HeadShape {
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// A vector of f32 values as two fp16 parts that sum to them (22 bits), held as
+// halves [128] and [128] in an LDS row.  Products of two such vectors take three
+// fp16 products (without low . low, 2^-22 of a term), where f32 MFMA takes 16
+// times one's time.  Normalised vectors are scaled by 2^kSplitExp and state rows
+// so that their largest value is about 2^kStateExp, which keeps the low parts
+// normal fp16 numbers.
+constexpr int kSplitExp = 8, kStateExp = 10;
+struct Split {
+    f16x8 hi, lo;
+};
+__device__ __forceinline__ Split split_row(const float *row, int at) {
+    const _Float16 *h = (const _Float16 *)row + at;
+    return {*(const f16x8 *)h, *(const f16x8 *)(h + 128)};
+}
+__device__ __forceinline__ f32x4 mma_split(const Split &a, const Split &b, f32x4 acc) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.lo, b.hi, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.lo, acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.hi, acc, 0, 0, 0);
+}
 
 // acc += A . B over 16 k: element i of both operands per instruction
 __device__ __forceinline__ f32x4 mma16(const f32x4 &a, const f32x4 &b, f32x4 acc) {
@@ -258,8 +279,8 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
     extern __shared__ __align__(16) float lds[];
     __shared__ double g_s[kRowsMax];
     __shared__ uint64_t anc_s[kRowsMax];
-    __shared__ float beta_s[kRowsMax], decay_s[kRowsMax], qn_s[kRowsMax], kn_s[kRowsMax];
-    __shared__ int tap_s[kRowsMax][8];
+    __shared__ float beta_s[kRowsMax], decay_s[kRowsMax];
+    __shared__ uint64_t tap_s[kRowsMax];  // LDS rows of a row's conv taps, a byte each, newest first
     float *xq = lds, *xk = lds + T::kPart, *xv = lds + 2 * T::kPart;
     float *As = lds + 3 * T::kPart, *Ps = As + T::kRows * kPair;
 
@@ -274,19 +295,22 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
     const uint32_t l16 = lane & 15, g4 = lane >> 4;
     float *rec = p.records + (size_t)m.slot * p.keep_rows * p.rec_stride;
 
-    // the wave's state rows: row 16 w + l16, dims 16 s + 4 g4 .. + 3
-    f32x4 S[8];
-    {
-        const float *src = p.state + (((size_t)m.state_in * p.value_heads + h) * kW + 16 * wave + l16) * kW + 4 * g4;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) S[s] = __builtin_nontemporal_load((const f32x4 *)(src + 16 * s));
-    }
     // 1.
     const uint32_t part = wave >> 1, c = tid & 127;  // q, k, v; waves 6 and 7 have no channel
     const uint32_t ch = part == 0 ? kh * kW + c
                       : part == 1 ? (p.key_heads + kh) * kW + c
                                   : 2 * p.key_heads * kW + h * kW + c;
     float *X = lds + part * T::kPart + c;
+    // the wave's state rows: row 16 w + l16, dims 32 s + 8 g4 .. + 7, requested behind the
+    // inputs, which are waited for first
+    f32x4 S[8];
+    auto load_state = [&]() __attribute__((always_inline)) {
+        const float *src = p.state + (((size_t)m.state_in * p.value_heads + h) * kW + 16 * wave + l16) * kW + 8 * g4;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            S[s] = __builtin_nontemporal_load((const f32x4 *)(src + 32 * (s >> 1) + 4 * (s & 1)));
+        }
+    };
     float w[8];
     if (part < 3) {
         const float *hist = p.history + (((size_t)m.parity * p.max_slots + m.slot) * p.channels + ch) * K1;
@@ -299,7 +323,9 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
 #pragma unroll
         for (uint32_t j = 0; j < kHist; ++j) old[j] = hist[j < K1 ? j : 0];
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) w[j] = p.conv_w[(size_t)ch * K + (j < K ? j : 0)];
+        for (uint32_t j = 0; j < 8; ++j) w[j] = p.conv_w[(size_t)ch * K + (j < K ? K1 - j : 0)];  // newest first
+        load_state();
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (uint32_t j = 0; j < kHist; ++j) {
             if (j < K1) X[(kHist - K1 + j) * kPitch] = old[j];
@@ -314,6 +340,8 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
         const uint32_t r = min(lane, R - 1);
         const float av = load_act(p.a, (size_t)(m.row0 + r) * p.value_heads + h, bf16);
         const float bv = load_act(p.b, (size_t)(m.row0 + r) * p.value_heads + h, bf16);
+        load_state();
+        __builtin_amdgcn_sched_barrier(0);
         const int up = (int)p.parent[m.row0 - p.meta[0].row0 + r] - 1;
         const float log_a = -expf(p.a_log[h]) * softplus_ref(av + p.dt_bias[h]);
         // the path's set and sum up to, not with, `next`: doubling
@@ -334,12 +362,14 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
             }
         }
         int at = (int)r, back = 0;
+        uint64_t taps = 0;
         for (uint32_t j = 0; j < K; ++j) {
             const int u = __shfl(up, at < 0 ? 0 : at);
-            if (lane < R) tap_s[lane][j] = at >= 0 ? (int)kHist + at : (int)kHist - 1 - back;
+            taps |= (uint64_t)(at >= 0 ? (int)kHist + at : (int)kHist - 1 - back) << (8 * j);
             back += at < 0 ? 1 : 0;
             at = at < 0 ? -1 : u;
         }
+        tap_s[lane] = taps;
         if (lane < R) {
             g_s[lane] = sum;
             anc_s[lane] = ((uint64_t)hi << 32) | lo;
@@ -350,59 +380,120 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
             // rows of the last tile past the tree
             g_s[lane] = 0.0;
             anc_s[lane] = 0;
-            beta_s[lane] = decay_s[lane] = qn_s[lane] = kn_s[lane] = 0.0f;
+            beta_s[lane] = decay_s[lane] = 0.0f;
         }
+    } else {
+        load_state();
     }
     __syncthreads();
     // 2. oldest tap first, as the reference sums them (math.rs:175-185)
     if (part < 3) {
-        for (int t0 = (int)R - 1; t0 >= 0; t0 -= 4) {
-            float acc[4];
+        auto conv = [&](auto taps_of) __attribute__((always_inline)) {
+            constexpr uint32_t KT = decltype(taps_of)::value;  // taps read per row
+            constexpr int kBatch = KT == 4 ? 8 : 4;            // rows whose reads are in flight
+            for (int t0 = (int)R - 1; t0 >= 0; t0 -= kBatch) {
+                float x[kBatch][KT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = max(t0 - i, 0);
-                acc[i] = 0.0f;
+                for (int i = 0; i < kBatch; ++i) {
+                    const uint64_t tap_v = tap_s[max(t0 - i, 0)];
+                    const uint32_t half[2] = {
+                        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)tap_v),
+                        KT > 4 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(tap_v >> 32)) : 0u};
 #pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) {
-                    if (j < K) acc[i] = fmaf(X[tap_s[t][K1 - j] * kPitch], w[j], acc[i]);
+                    for (uint32_t j = 0; j < KT; ++j) {
+                        // (past the kernel's taps: row 0, unused)
+                        const uint32_t row = (half[j >> 2] >> (8 * (j & 3))) & 255u;
+                        x[i][j] = X[row * kPitch];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    float acc = 0.0f;
+#pragma unroll
+                    for (uint32_t j = 0; j < KT; ++j) {
+                        const uint32_t back = KT - 1 - j;
+                        if (back < K) acc = fmaf(x[i][back], w[back], acc);
+                    }
+                    if (t0 - i >= 0) X[(kHist + t0 - i) * kPitch] = silu_fast(acc);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (t0 - i >= 0) X[(kHist + t0 - i) * kPitch] = silu_fast(acc[i]);
-            }
-        }
+        };
+        if (K == 4) conv(std::integral_constant<uint32_t, 4>{});
+        else conv(std::integral_constant<uint32_t, 8>{});
     }
     __syncthreads();
-    // 3.
-    for (uint32_t t = wave; t < 2 * R; t += 8) {
-        const float *y = ((t & 1) ? xk : xq) + (kHist + (t >> 1)) * kPitch;
-        const float y0 = y[lane], y1 = y[lane + 64];
-        const float ss = sum64(fmaf(y1, y1, y0 * y0));
-        const float inv = 1.0f / sqrtf(ss + 1e-6f);
-        if (lane == 0) ((t & 1) ? kn_s : qn_s)[t >> 1] = inv;
-        if ((t & 1) && first_of_key) {
-            float *key = rec + (size_t)(t >> 1) * p.rec_stride + rec_key(p) + kh * kW;
-            key[lane] = y0 * inv;
-            key[lane + 64] = y1 * inv;
+    // 3. four vectors of a wave at a time
+    for (uint32_t t0 = wave; t0 < 2 * R; t0 += 32) {
+        float2 y[4];
+        float inv[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t t = min(t0 + 8 * i, 2 * R - 1);
+            y[i] = *(const float2 *)(((t & 1) ? xk : xq) + (kHist + (t >> 1)) * kPitch + 2 * lane);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            inv[i] = 1.0f / sqrtf(sum64(fmaf(y[i].y, y[i].y, y[i].x * y[i].x)) + 1e-6f);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t t = t0 + 8 * i;
+            if (t >= 2 * R) break;
+            const float a = y[i].x * inv[i], b = y[i].y * inv[i];
+            if ((t & 1) && first_of_key) {
+                *(float2 *)(rec + (size_t)(t >> 1) * p.rec_stride + rec_key(p) + kh * kW + 2 * lane) = make_float2(a, b);
+            }
+            constexpr float kScale = (float)(1 << kSplitExp);
+            const f16x2 hi = {(_Float16)(a * kScale), (_Float16)(b * kScale)};
+            const f16x2 lo = {(_Float16)(a * kScale - (float)hi.x), (_Float16)(b * kScale - (float)hi.y)};
+            f16x2 *row = (f16x2 *)(((t & 1) ? xk : xq) + (kHist + (t >> 1)) * kPitch);
+            row[lane] = hi;
+            row[64 + lane] = lo;
         }
     }
+    // the state rows' parts
+    Split Sp[4];
+    int back;  // exponent that undoes the scales
+    {
+        float mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fabsf(S[s][i]));
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        // (frexp's exponent: max in [2^(e - 1), 2^e); 0 for 0)
+        const int up = kStateExp - __builtin_amdgcn_frexp_expf(mx);
+        back = -up - kSplitExp;
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = __builtin_amdgcn_ldexpf(S[s][i], up);
+                const _Float16 hi = (_Float16)x;
+                Sp[s >> 1].hi[4 * (s & 1) + i] = hi;
+                Sp[s >> 1].lo[4 * (s & 1) + i] = (_Float16)(x - (float)hi);
+            }
+    }
+    __syncthreads();
     // 4.
     f32x4 kS[RT], qS[RT];
 #pragma unroll
-    for (int b = 0; b < RT; ++b) kS[b] = qS[b] = f32x4{};
-#pragma unroll
     for (int b = 0; b < RT; ++b) {
-        if ((uint32_t)b >= rt) break;
-        const float *kr = xk + (kHist + 16 * b + l16) * kPitch + 4 * g4;
-        const float *qr = xq + (kHist + 16 * b + l16) * kPitch + 4 * g4;
+        kS[b] = qS[b] = f32x4{};
+        if ((uint32_t)b >= rt) continue;
+        const float *kr = xk + (kHist + 16 * b + l16) * kPitch, *qr = xq + (kHist + 16 * b + l16) * kPitch;
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            kS[b] = mma16(*(const f32x4 *)(kr + 16 * s), S[s], kS[b]);
-            qS[b] = mma16(*(const f32x4 *)(qr + 16 * s), S[s], qS[b]);
+        for (int s = 0; s < 4; ++s) {
+            kS[b] = mma_split(split_row(kr, 32 * s + 8 * g4), Sp[s], kS[b]);
+            qS[b] = mma_split(split_row(qr, 32 * s + 8 * g4), Sp[s], qS[b]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            kS[b][e] = __builtin_amdgcn_ldexpf(kS[b][e], back);
+            qS[b][e] = __builtin_amdgcn_ldexpf(qS[b][e], back);
         }
     }
-    __syncthreads();
     {
         // blocks (bt, bj), bj <= bt, of K K^T, then of Q K^T
         const uint32_t blocks = rt * (rt + 1);
@@ -410,24 +501,23 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
             const bool is_q = i >= blocks / 2;
             uint32_t bj = is_q ? i - blocks / 2 : i, bt = 0;
             while (bj > bt) bj -= ++bt;
-            const float *ar = (is_q ? xq : xk) + (kHist + 16 * bt + l16) * kPitch + 4 * g4;
-            const float *br = xk + (kHist + 16 * bj + l16) * kPitch + 4 * g4;
+            const float *ar = (is_q ? xq : xk) + (kHist + 16 * bt + l16) * kPitch;
+            const float *br = xk + (kHist + 16 * bj + l16) * kPitch;
             f32x4 acc[2] = {f32x4{}, f32x4{}};
 #pragma unroll
-            for (int s = 0; s < 8; ++s) {
-                acc[s & 1] = mma16(*(const f32x4 *)(ar + 16 * s), *(const f32x4 *)(br + 16 * s), acc[s & 1]);
+            for (int s = 0; s < 4; ++s) {
+                acc[s & 1] = mma_split(split_row(ar, 32 * s + 8 * g4), split_row(br, 32 * s + 8 * g4), acc[s & 1]);
             }
             const uint32_t j = 16 * bj + l16;
             const double gj = g_s[j];
-            const float kj = kn_s[j];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint32_t t = 16 * bt + 4 * g4 + e;
                 const bool sees = (anc_s[t] >> j) & 1;
                 const float ratio = __builtin_amdgcn_exp2f((float)(g_s[t] - gj) * kLog2e);
-                const float dot = (acc[0][e] + acc[1][e]) * kj;
-                if (is_q) Ps[t * kPair + j] = sees ? dot * qn_s[t] * ratio : 0.0f;
-                else As[t * kPair + j] = sees && t != j ? -dot * kn_s[t] * ratio * beta_s[t] : 0.0f;
+                const float dot = (acc[0][e] + acc[1][e]) * (1.0f / (1 << (2 * kSplitExp)));
+                if (is_q) Ps[t * kPair + j] = sees ? dot * ratio : 0.0f;
+                else As[t * kPair + j] = sees && t != j ? -dot * ratio * beta_s[t] : 0.0f;
             }
         }
     }
@@ -471,8 +561,8 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const uint32_t t = 16 * b + 4 * g4 + e;
-            rhs[e] = beta_s[t] * (vr[e * kPitch] - decay_s[t] * kn_s[t] * kS[b][e]);
-            o[e] = decay_s[t] * qn_s[t] * qS[b][e];
+            rhs[e] = beta_s[t] * (vr[e * kPitch] - decay_s[t] * kS[b][e]);
+            o[e] = decay_s[t] * qS[b][e];
         }
         const float *Ar = As + (16 * b + l16) * kPair + 4 * g4;
         const float *Pr = Ps + (16 * b + l16) * kPair + 4 * g4;
