@@ -260,6 +260,15 @@ __device__ __forceinline__ f32x4 mma_split(const Split &a, const Split &b, f32x4
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.hi, acc, 0, 0, 0);
 }
 
+// Sum over the wave, without LDS.
+__device__ __forceinline__ float wave_sum(float x) {
+    x = sum16(x);
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_int(x), __float_as_int(x), false, false);
+    x = __int_as_float(r[0]) + __int_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_int(x), __float_as_int(x), false, false);
+    return __int_as_float(r[0]) + __int_as_float(r[1]);
+}
+
 // acc += A . B over 16 k: element i of both operands per instruction
 __device__ __forceinline__ f32x4 mma16(const f32x4 &a, const f32x4 &b, f32x4 acc) {
 #pragma unroll
@@ -280,7 +289,8 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
     __shared__ double g_s[kRowsMax];
     __shared__ uint64_t anc_s[kRowsMax];
     __shared__ float beta_s[kRowsMax], decay_s[kRowsMax];
-    __shared__ uint64_t tap_s[kRowsMax];  // LDS rows of a row's conv taps, a byte each, newest first
+    // a row's conv taps, newest first: byte offsets of their LDS rows
+    __shared__ __align__(16) uint16_t tap_s[kRowsMax][8];
     float *xq = lds, *xk = lds + T::kPart, *xv = lds + 2 * T::kPart;
     float *As = lds + 3 * T::kPart, *Ps = As + T::kRows * kPair;
 
@@ -323,7 +333,10 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
 #pragma unroll
         for (uint32_t j = 0; j < kHist; ++j) old[j] = hist[j < K1 ? j : 0];
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) w[j] = p.conv_w[(size_t)ch * K + (j < K ? K1 - j : 0)];  // newest first
+        for (uint32_t j = 0; j < 8; ++j) {
+            const float x = p.conv_w[(size_t)ch * K + (j < K ? K1 - j : 0)];  // newest first
+            w[j] = j < K ? x : 0.0f;
+        }
         load_state();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -362,14 +375,16 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
             }
         }
         int at = (int)r, back = 0;
-        uint64_t taps = 0;
-        for (uint32_t j = 0; j < K; ++j) {
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) {
+            // past the kernel's taps: any finite row, its weight is 0
+            if (j >= K) at = (int)r;
+            if (lane >= R) at = (int)lane;
             const int u = __shfl(up, at < 0 ? 0 : at);
-            taps |= (uint64_t)(at >= 0 ? (int)kHist + at : (int)kHist - 1 - back) << (8 * j);
+            tap_s[lane][j] = (uint16_t)((at >= 0 ? (int)kHist + at : (int)kHist - 1 - back) * (int)(kPitch * 4));
             back += at < 0 ? 1 : 0;
             at = at < 0 ? -1 : u;
         }
-        tap_s[lane] = taps;
         if (lane < R) {
             g_s[lane] = sum;
             anc_s[lane] = ((uint64_t)hi << 32) | lo;
@@ -385,70 +400,78 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
     } else {
         load_state();
     }
+    // 8. barrier
     __syncthreads();
-    // 2. oldest tap first, as the reference sums them (math.rs:175-185)
+    // 2. oldest tap first, as the reference sums them (math.rs:175-185); rows past the
+    // tree are zeros with themselves as taps
     if (part < 3) {
         auto conv = [&](auto taps_of) __attribute__((always_inline)) {
             constexpr uint32_t KT = decltype(taps_of)::value;  // taps read per row
             constexpr int kBatch = KT == 4 ? 8 : 4;            // rows whose reads are in flight
-            for (int t0 = (int)R - 1; t0 >= 0; t0 -= kBatch) {
+            for (int t0 = 16 * (int)rt - kBatch; t0 >= 0; t0 -= kBatch) {
+                uint32_t tap[kBatch][KT / 2];
                 float x[kBatch][KT];
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i) {
-                    const uint64_t tap_v = tap_s[max(t0 - i, 0)];
-                    const uint32_t half[2] = {
-                        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)tap_v),
-                        KT > 4 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(tap_v >> 32)) : 0u};
+                for (int i = 0; i < kBatch; ++i)
 #pragma unroll
-                    for (uint32_t j = 0; j < KT; ++j) {
-                        // (past the kernel's taps: row 0, unused)
-                        const uint32_t row = (half[j >> 2] >> (8 * (j & 3))) & 255u;
-                        x[i][j] = X[row * kPitch];
+                    for (uint32_t j = 0; j < KT / 2; ++j) tap[i][j] = ((const uint32_t *)tap_s[t0 + i])[j];
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+                    for (uint32_t j = 0; j < KT / 2; ++j) {
+                        const uint32_t two = (uint32_t)__builtin_amdgcn_readfirstlane((int)tap[i][j]);
+                        x[i][2 * j] = *(const float *)((const char *)X + (two & 0xffffu));
+                        x[i][2 * j + 1] = *(const float *)((const char *)X + (two >> 16));
                     }
-                }
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < kBatch; ++i) {
                     float acc = 0.0f;
 #pragma unroll
                     for (uint32_t j = 0; j < KT; ++j) {
-                        const uint32_t back = KT - 1 - j;
-                        if (back < K) acc = fmaf(x[i][back], w[back], acc);
+                        // (weights past the kernel's are 0)
+                        acc = fmaf(x[i][KT - 1 - j], w[KT - 1 - j], acc);
                     }
-                    if (t0 - i >= 0) X[(kHist + t0 - i) * kPitch] = silu_fast(acc);
+                    x[i][0] = acc;
                 }
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) X[(kHist + t0 + i) * kPitch] = silu_fast(x[i][0]);
             }
         };
-        if (K == 4) conv(std::integral_constant<uint32_t, 4>{});
+        if (K <= 4) conv(std::integral_constant<uint32_t, 4>{});
         else conv(std::integral_constant<uint32_t, 8>{});
     }
     __syncthreads();
-    // 3. four vectors of a wave at a time
+    // 3. four vectors of a wave at a time; past the last, the last again
     for (uint32_t t0 = wave; t0 < 2 * R; t0 += 32) {
         float2 y[4];
         float inv[4];
+        float *row[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t t = min(t0 + 8 * i, 2 * R - 1);
-            y[i] = *(const float2 *)(((t & 1) ? xk : xq) + (kHist + (t >> 1)) * kPitch + 2 * lane);
+            const uint32_t t = min(t0 + 8 * i, (t0 & 1) + 2 * R - 2);
+            row[i] = ((t & 1) ? xk : xq) + (kHist + (t >> 1)) * kPitch;
+            y[i] = *(const float2 *)(row[i] + 2 * lane);
         }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) inv[i] = fmaf(y[i].y, y[i].y, y[i].x * y[i].x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) inv[i] = __builtin_amdgcn_rsqf(wave_sum(inv[i]) + 1e-6f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            inv[i] = 1.0f / sqrtf(sum64(fmaf(y[i].y, y[i].y, y[i].x * y[i].x)) + 1e-6f);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t t = t0 + 8 * i;
-            if (t >= 2 * R) break;
             const float a = y[i].x * inv[i], b = y[i].y * inv[i];
-            if ((t & 1) && first_of_key) {
-                *(float2 *)(rec + (size_t)(t >> 1) * p.rec_stride + rec_key(p) + kh * kW + 2 * lane) = make_float2(a, b);
-            }
             constexpr float kScale = (float)(1 << kSplitExp);
             const f16x2 hi = {(_Float16)(a * kScale), (_Float16)(b * kScale)};
             const f16x2 lo = {(_Float16)(a * kScale - (float)hi.x), (_Float16)(b * kScale - (float)hi.y)};
-            f16x2 *row = (f16x2 *)(((t & 1) ? xk : xq) + (kHist + (t >> 1)) * kPitch);
-            row[lane] = hi;
-            row[64 + lane] = lo;
+            if (t0 + 8 * i < 2 * R) {
+                ((f16x2 *)row[i])[lane] = hi;
+                ((f16x2 *)row[i])[64 + lane] = lo;
+                if ((t0 & 1) && first_of_key) {
+                    *(float2 *)(rec + (size_t)((t0 + 8 * i) >> 1) * p.rec_stride + rec_key(p) + kh * kW + 2 * lane) = make_float2(a, b);
+                }
+            }
         }
     }
     // the state rows' parts
@@ -581,20 +604,34 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
         }
     }
     __syncthreads();
-    // 7. RMSNorm without offset, then * silu(z) (native.rs:737-740)
+    // 7. RMSNorm without offset, then * silu(z) (native.rs:737-740); rows past the
+    // wave's last repeat it
     const float n0 = p.norm[lane], n1 = p.norm[lane + 64];
+    constexpr int kOut = 2 * RT < 4 ? 2 * RT : 4;  // rows at a time
 #pragma unroll
-    for (int i = 0; i < 2 * RT; ++i) {
-        const uint32_t t = wave + 8 * i;
-        if (t >= R) break;
-        const float *o = xv + (kHist + t) * kPitch;
-        const float o0 = o[lane], o1 = o[lane + 64];
-        const float variance = sum64(fmaf(o1, o1, o0 * o0)) / (float)kW;
-        if (!isfinite(variance) && lane == 0) atomicOr(p.err_word, kErrNonFiniteVariance);
-        const float inv = 1.0f / sqrtf(variance + p.eps);
-        float *dst = p.out + (size_t)(m.row0 + t) * width + h * kW;
-        dst[lane] = o0 * inv * n0 * silu_fast(z0[i]);
-        dst[lane + 64] = o1 * inv * n1 * silu_fast(z1[i]);
+    for (int i0 = 0; i0 < 2 * RT; i0 += kOut) {
+        if (wave + 8 * i0 >= R) break;
+        float o0[kOut], o1[kOut], inv[kOut];
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) {
+            const float *o = xv + (kHist + min(wave + 8 * (i0 + i), R - 1)) * kPitch;
+            o0[i] = o[lane];
+            o1[i] = o[lane + 64];
+        }
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) {
+            const float variance = wave_sum(fmaf(o1[i], o1[i], o0[i] * o0[i])) / (float)kW;
+            if (!isfinite(variance) && lane == 0) atomicOr(p.err_word, kErrNonFiniteVariance);
+            inv[i] = 1.0f / sqrtf(variance + p.eps);
+        }
+#pragma unroll
+        for (int i = 0; i < kOut; ++i) {
+            const uint32_t t = wave + 8 * (i0 + i);
+            if (t >= R) break;
+            float *dst = p.out + (size_t)(m.row0 + t) * width + h * kW;
+            dst[lane] = o0[i] * inv[i] * n0 * silu_fast(z0[i0 + i]);
+            dst[lane + 64] = o1[i] * inv[i] * n1 * silu_fast(z1[i0 + i]);
+        }
     }
 }
 
