@@ -16,6 +16,7 @@
 //                        applies the output gate.
 // tree_generic_kernel takes the head widths other than 64, 128 and 256.
 #include <algorithm>
+#include <type_traits>
 
 #include "sr_device.hpp"
 #include "tree_plan.hpp"
@@ -357,11 +358,12 @@ __global__ void __launch_bounds__(64) tree_generic_kernel(const TreeCommon c) {
 //
 // A workgroup has up to 4 x 32 query vectors and 32 KB stages of kKeys keys: a
 // wave takes one of the vector groups and 32 keys of a stage.  Stages come
-// straight into LDS (global_load_lds, 16 bytes per lane), kStages - 1 ahead, one
+// straight into LDS (global_load_lds, 16 bytes per lane), kAhead ahead, one
 // barrier per stage; a row's 16-byte units are swapped by its index so that the
 // operand reads (ds_read_b128 of K, ds_read_b64_tr_b16 of V) meet no bank twice.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kStages = 4;
+constexpr uint32_t kAhead = 2;  // stages on their way; one more may still be read by late waves
 constexpr uint32_t kStageBytes = 32768;
 constexpr float kLazy = 8.0f;  // log2 growth of the maximum before sums are rescaled
 
@@ -391,59 +393,37 @@ template <int D>
 __device__ __forceinline__ uint32_t k_unit(uint32_t r, uint32_t u) {
     return D == 64 ? u ^ ((r >> 1) & 7) : u ^ (r & 15);
 }
-template <int D>
-__device__ __forceinline__ uint32_t v_unit(uint32_t r, uint32_t u) {
-    return D == 64 ? u ^ (((r >> 1) & 1) << 2) : u ^ ((r & 3) << 2);
-}
-
-// Operands of O^T += V^T P^T for keys 16 st .. of a wave's 32: lane (d = lane & 31
-// of a 32-dim tile, h) gets V[16 st + 4 h + {0..3, 8..11}][d] by two transposing
-// reads per tile.  Written out with their wait: the builtin's reads would wait for
-// every stage that is still on its way into LDS.
+// A lane's dims of one key row of V: D / 32 bf16 values, dims D / 32 i .. of lane i.
+// (A vector type, read as such: the compiler takes reads through it, unlike reads of
+// integers or structs, for apart from the stages on their way into LDS and does not
+// wait for those.)
 template <int NT>
-struct VFrag {
-    uint2 lo[NT], hi[NT];
-    __device__ __forceinline__ bf16x8 get(int t) const {
-        return __builtin_bit_cast(bf16x8, u32x4{lo[t].x, lo[t].y, hi[t].x, hi[t].y});
-    }
+struct VRowOf {
+    typedef __bf16 type __attribute__((ext_vector_type(NT)));
 };
-template <int D, int ST>
-__device__ __forceinline__ void read_v(VFrag<4> &f, const uint32_t (&a)[4]) {
-    constexpr int kLo = ST * 16 * D * 2, kHi = kLo + 8 * D * 2;
-    asm volatile(
-        "ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %4, %8 offset:%13\n\t"
-        "ds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
-        "ds_read_b64_tr_b16 %2, %10 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %6, %10 offset:%13\n\t"
-        "ds_read_b64_tr_b16 %3, %11 offset:%12\n\t"
-        "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(f.lo[0]), "=&v"(f.lo[1]), "=&v"(f.lo[2]), "=&v"(f.lo[3]), "=&v"(f.hi[0]),
-          "=&v"(f.hi[1]), "=&v"(f.hi[2]), "=&v"(f.hi[3])
-        : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(kLo), "n"(kHi)
-        : "memory");
-}
-template <int D, int ST>
-__device__ __forceinline__ void read_v(VFrag<2> &f, const uint32_t (&a)[2]) {
-    constexpr int kLo = ST * 16 * D * 2, kHi = kLo + 8 * D * 2;
-    asm volatile(
-        "ds_read_b64_tr_b16 %0, %4 offset:%6\n\t"
-        "ds_read_b64_tr_b16 %2, %4 offset:%7\n\t"
-        "ds_read_b64_tr_b16 %1, %5 offset:%6\n\t"
-        "ds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(f.lo[0]), "=&v"(f.lo[1]), "=&v"(f.hi[0]), "=&v"(f.hi[1])
-        : "v"(a[0]), "v"(a[1]), "n"(kLo), "n"(kHi)
-        : "memory");
+template <int NT>
+using VRow = typename VRowOf<NT>::type;
+// Operand of O^T += V^T P^T for tile t (row i: dim NT i + t) from 8 keys' rows: the
+// keys' values of that dim, two to a register.
+template <int NT>
+__device__ __forceinline__ bf16x8 v_operand(const VRow<NT> (&v)[8], int t) {
+    struct Words {
+        uint32_t w[NT / 2];
+    };
+    u32x4 x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        x[j] = __builtin_amdgcn_perm(__builtin_bit_cast(Words, v[2 * j + 1]).w[t / 2],
+                                     __builtin_bit_cast(Words, v[2 * j]).w[t / 2],
+                                     (t & 1) ? 0x07060302u : 0x05040100u);
+    }
+    return __builtin_bit_cast(bf16x8, x);
 }
 
 template <int D, int VG, bool kF32>
 __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_kernel(const TreeCommon c) {
     using T = TreeShape<D, VG, kF32>;
     constexpr int NS = D / 16, NT = D / 32;
-    constexpr int TPG = NT < 4 ? NT : 4;  // 32-dim tiles per group of V reads
     constexpr int CH = D / 8;             // 16-byte units per row
     constexpr int RPI = 64 / CH;          // rows per load instruction
     constexpr int kLoads = 16 / T::NW > 0 ? 16 / T::NW : 1;  // of K, and of V, per wave and stage
@@ -475,39 +455,9 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
     const uint32_t key_end = min(key_begin + c.part_keys, m.ctx + m.rows);  // > key_begin
     const uint32_t steps = (key_end - key_begin + T::kKeys - 1) / T::kKeys;
 
-    // page ids of the partition
-    const uint32_t lpt = c.log2_page, pmask = (1u << lpt) - 1;
-    const uint32_t first_page = key_begin >> lpt;
-    const uint32_t npages = ((key_end - 1) >> lpt) - first_page + 1;
-    const int32_t *table = c.page_table + (size_t)m.slot * c.pages_per_seq + first_page;
-    for (uint32_t i = tid; i < npages; i += T::kThreads) pids[i] = table[i];
-    __syncthreads();
-
-    // stage k into its buffer: load i of a wave covers rows RPI (wave + NW i) .. of K
-    // and of V.  Rows past the last key load it again: they are masked, and finite.
-    const unsigned char *k_head = (const unsigned char *)c.k_pages + (((size_t)kvh * c.num_pages) << lpt) * (D * 2);
-    const unsigned char *v_head = (const unsigned char *)c.v_pages + (((size_t)kvh * c.num_pages) << lpt) * (D * 2);
-    const uint32_t lrow = lane / CH, lunit = lane % CH;
-    auto issue = [&](uint32_t k) __attribute__((always_inline)) {
-        unsigned char *buf = lds + (k % kStages) * kStageBytes;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const uint32_t r0 = RPI * (wave + T::NW * i);
-            const uint32_t key0 = key_begin + k * T::kKeys + r0;
-            const uint32_t base = min(key0, (key_end - 1) & ~(uint32_t)(RPI - 1));
-            const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane(pids[(base >> lpt) - first_page]);
-            const uint32_t tok = min(base + lrow, key_end - 1);
-            const size_t row = (((size_t)page << lpt) + (tok & pmask)) * (D * 2);
-            const uint32_t r = r0 + lrow;
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void *)(k_head + row + k_unit<D>(r, lunit) * 16),
-                (__attribute__((address_space(3))) void *)(buf + r0 * (D * 2)), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void *)(v_head + row + v_unit<D>(r, lunit) * 16),
-                (__attribute__((address_space(3))) void *)(buf + kStageBytes / 2 + r0 * (D * 2)), 16, 0, 0);
-        }
-    };
-    // this wave's query vectors (its first one at least exists, or it only loads)
+    // this wave's query vectors (a wave without any only loads keys).  They are
+    // requested ahead of the page ids, so that nothing of theirs is on its way when the
+    // stages are: the compiler would wait for those too, in every step
     const uint32_t col = lane & 31, h = lane >> 5;
     const uint32_t tiles = (nvec + 31) / 32;
     const uint32_t tile = slice * VG + vg;
@@ -523,10 +473,66 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
 #pragma unroll
             for (int st = 0; st < NS; ++st) q[p][st] = __builtin_bit_cast(bf16x8, src[(p * NS + st) * 64]);
     }
-    const uint4 mask = c.masks[m.row0 + row];
-    const uint64_t mask_lo = ((uint64_t)mask.y << 32) | mask.x, mask_hi = ((uint64_t)mask.w << 32) | mask.z;
+    uint4 mask = c.masks[m.row0 + row];
 
-    for (uint32_t k = 0; k + 1 < kStages; ++k) {
+    // page ids of the partition
+    const uint32_t lpt = c.log2_page, pmask = (1u << lpt) - 1;
+    const uint32_t first_page = key_begin >> lpt;
+    const uint32_t npages = ((key_end - 1) >> lpt) - first_page + 1;
+    const int32_t *table = c.page_table + (size_t)m.slot * c.pages_per_seq + first_page;
+    for (uint32_t i = tid; i < npages; i += T::kThreads) pids[i] = table[i];
+#pragma unroll
+    for (int p = 0; p < T::QP; ++p)
+#pragma unroll
+        for (int st = 0; st < NS; ++st) asm volatile("" : "+v"(q[p][st]));  // arrived
+    asm volatile("" : "+v"(mask.x), "+v"(mask.y), "+v"(mask.z), "+v"(mask.w));
+    const uint64_t mask_lo = ((uint64_t)mask.y << 32) | mask.x, mask_hi = ((uint64_t)mask.w << 32) | mask.z;
+    __syncthreads();
+
+    // stage k into its buffer: load i of a wave covers rows RPI (wave + NW i) .. of K
+    // and of V.  Rows past the last key load it again: they are masked, and finite.
+    const unsigned char *k_head = (const unsigned char *)c.k_pages + (((size_t)kvh * c.num_pages) << lpt) * (D * 2);
+    const unsigned char *v_head = (const unsigned char *)c.v_pages + (((size_t)kvh * c.num_pages) << lpt) * (D * 2);
+    const uint32_t lrow = lane / CH, lunit = lane % CH;
+    // a wave's page ids of the next stage to issue, read from LDS a stage ahead
+    int32_t ahead[kLoads];
+    auto page_ids = [&](uint32_t k) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t key0 = key_begin + k * T::kKeys + RPI * (wave + T::NW * i);
+            ahead[i] = pids[(min(key0, key_end - 1) >> lpt) - first_page];
+        }
+    };
+    auto to_lds = [](const unsigned char *from, unsigned char *to) __attribute__((always_inline)) {
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)from,
+                                         (__attribute__((address_space(3))) void *)to, 16, 0, 0);
+    };
+    auto issue = [&](uint32_t k) __attribute__((always_inline)) {
+        unsigned char *buf = lds + (k % kStages) * kStageBytes;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t r0 = RPI * (wave + T::NW * i);
+            const uint32_t key0 = key_begin + k * T::kKeys + r0;
+            const uint32_t page = (uint32_t)__builtin_amdgcn_readfirstlane(ahead[i]);
+            unsigned char *to = buf + r0 * (D * 2);
+            if (key0 + RPI <= key_end) {
+                // (rows r0 .. are in one page: a page holds at least 16 keys)
+                const size_t at = (((size_t)page << lpt) + (key0 & pmask)) * (D * 2);
+                const uint32_t r = r0 + lrow;
+                to_lds(k_head + at + (lrow * (D * 2) + k_unit<D>(r, lunit) * 16), to);
+                to_lds(v_head + at + (lrow * (D * 2) + lunit * 16), to + kStageBytes / 2);
+            } else {
+                const uint32_t base = min(key0, (key_end - 1) & ~(uint32_t)(RPI - 1));
+                const uint32_t tok = min(base + lrow, key_end - 1), r = r0 + lrow;
+                const size_t at = (((size_t)page << lpt) + (tok & pmask)) * (D * 2);
+                to_lds(k_head + at + k_unit<D>(r, lunit) * 16, to);
+                to_lds(v_head + at + lunit * 16, to + kStageBytes / 2);
+            }
+        }
+        page_ids(k + 1);
+    };
+    page_ids(0);
+    for (uint32_t k = 0; k < kAhead; ++k) {
         if (k < steps) issue(k);
     }
 
@@ -534,42 +540,43 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t] = f32x16{};
     float m_run = -INFINITY, l_run = 0.0f;
-    // LDS addresses of V's transposing reads (k-step 0, first four rows)
-    uint32_t v_at[NT];
-    {
-        const uint32_t i16 = lane & 15, g = lane >> 4;
-        const uint32_t r = 4 * (g >> 1) + (i16 >> 2);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const uint32_t u = 4 * t + ((g & 1) << 1) + ((i16 >> 1) & 1);
-            v_at[t] = kStageBytes / 2 + (32 * kg + r) * (D * 2) + v_unit<D>(r, u) * 16 + (i16 & 1) * 8;
-        }
-    }
-    for (uint32_t k = 0; k < steps; ++k) {
+    // the beginning of step k
+    auto enter = [&](uint32_t k) __attribute__((always_inline)) {
         // this wave's loads of stage k have landed when at most those of the
         // stages after it are outstanding
-        constexpr int kPer = 2 * kLoads;
-        const uint32_t after = min(steps - 1 - k, kStages - 2);
-        if (after >= 2) __builtin_amdgcn_s_waitcnt(0x0F70 | ((2 * kPer > 63 ? 63 : 2 * kPer) & 15) | (((2 * kPer > 63 ? 63 : 2 * kPer) >> 4) << 14));
-        else if (after == 1) __builtin_amdgcn_s_waitcnt(0x0F70 | (kPer & 15) | ((kPer >> 4) << 14));
+        constexpr int kPer = 2 * kLoads < 64 ? 2 * kLoads : 63;
+        if (k + 1 < steps) __builtin_amdgcn_s_waitcnt(0x0F70 | (kPer & 15) | ((kPer >> 4) << 14));
         else __builtin_amdgcn_s_waitcnt(0x0F70);
-        // every wave's loads of stage k have landed, and the buffer of stage k - 1
+        // every wave's loads of stage k have landed, and the buffer of stage k - 2
         // has been read
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (k + kStages - 1 < steps) issue(k + kStages - 1);
-        const uint32_t key0 = key_begin + k * T::kKeys + 32 * kg;
-        if (!live || key0 >= key_end) continue;
-        const unsigned char *buf = lds + (k % kStages) * kStageBytes;
-        const unsigned char *kt = buf + 32 * kg * (D * 2);
-        f32x16 sacc{};
+        if (k + kAhead < steps) issue(k + kAhead);
+    };
+    // a wave has its SIMD to itself
+    constexpr bool kAlone = T::NW <= 4;
+    // steps st0 .. st1 - 1 of the scores of stage k; a wave alone keeps two chains of
+    // products going
+    constexpr int kChains = kAlone ? 2 : 1;
+    auto scores = [&](uint32_t k, int st0, int st1, f32x16 (&acc)[kChains]) __attribute__((always_inline)) {
+        const unsigned char *kt = lds + (k % kStages) * kStageBytes + 32 * kg * (D * 2);
 #pragma unroll
-        for (int st = 0; st < NS; ++st) {
+        for (int st = st0; st < st1; ++st) {
             const bf16x8 a = *(const bf16x8 *)(kt + col * (D * 2) + k_unit<D>(col, 2 * st + h) * 16);
 #pragma unroll
-            for (int p = 0; p < T::QP; ++p) sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[p][st], sacc, 0, 0, 0);
+            for (int p = 0; p < T::QP; ++p) {
+                f32x16 &x = acc[(st + p) % kChains];
+                x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[p][st], x, 0, 0, 0);
+            }
         }
+    };
+    // One stage's softmax and P V, with the scores of the next beside them: the
+    // matrix instructions run while the vector ones are issued.
+    f32x16 held;  // scores of stage k - 1
+    auto advance = [&](uint32_t k, auto next_of) __attribute__((always_inline)) {
+        constexpr bool kNext = decltype(next_of)::value;
+        const uint32_t key0 = key_begin + (k - 1) * T::kKeys + 32 * kg;
         if (key0 + 32 > m.ctx) {
             // bits of the wave's 32 keys: context keys, and the row's ancestors
             uint32_t w;
@@ -585,9 +592,11 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
             w >>= 4 * h;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                if (!((w >> (8 * (i >> 2) + (i & 3))) & 1u)) sacc[i] = -INFINITY;
+                if (!((w >> (8 * (i >> 2) + (i & 3))) & 1u)) held[i] = -INFINITY;
             }
         }
+        f32x16 acc[kChains] = {};
+        if constexpr (kNext) scores(k, 0, NS / 4, acc);
         // d = s - reference.  The reference only moves when the maximum outgrows it by
         // kLazy (or at the first visible key): sums and outputs are the same for any
         // common shift, and rescaling is rare.  (The maximum is of differences: of
@@ -595,7 +604,7 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
         float ref = m_run == -INFINITY ? 0.0f : m_run;
         float d[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) d[i] = sacc[i] - ref;
+        for (int i = 0; i < 16; ++i) d[i] = held[i] - ref;
         float mx = fmaxf(fmaxf(fmaxf(d[0], d[1]), d[2]), fmaxf(fmaxf(d[3], d[4]), d[5]));
         mx = fmaxf(fmaxf(mx, d[6]), fmaxf(fmaxf(d[7], d[8]), d[9]));
         mx = fmaxf(fmaxf(mx, d[10]), fmaxf(fmaxf(d[11], d[12]), d[13]));
@@ -607,17 +616,44 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
             m_run = next;
             ref = next == -INFINITY ? 0.0f : next;
             l_run *= scale;
+            if constexpr (kAlone) {
+                // a wave with the whole register file keeps o in accumulation registers;
+                // multiplied there, or the compiler moves all of it back and forth in
+                // every step.  (The wait: the last products' results, 18 cycles.)
+                asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) o[t][i] *= scale;
+                    for (int i = 0; i < 16; ++i) {
+                        float x;
+                        asm volatile("v_accvgpr_read_b32 %1, %0\n\ts_nop 1\n\tv_mul_f32 %1, %1, %2\n\ts_nop 1\n\t"
+                                     "v_accvgpr_write_b32 %0, %1\n\ts_nop 1"
+                                     : "+a"(o[t][i]), "=&v"(x)
+                                     : "v"(scale));
+                    }
+                asm volatile("s_nop 7" ::: "memory");
+            } else {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) d[i] = sacc[i] - ref;
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[t][i] *= scale;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) d[i] = held[i] - ref;
         }
-        bf16x8 p[T::PP][2];
+        // V rows of the wave's keys: lane (i, h) reads its dims of keys 16 st + 4 h +
+        // {0..3, 8..11}, those of its probabilities
+        const unsigned char *vt = lds + ((k - 1) % kStages) * kStageBytes + kStageBytes / 2 +
+                                  (32 * kg + 4 * h) * (D * 2) + col * (NT * 2);
         float sum[4] = {};
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
+            VRow<NT> v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = *(const VRow<NT> *)(vt + (16 * st + (j & 3) + 8 * (j >> 2)) * (D * 2));
+            }
+            if constexpr (kNext) scores(k, NS / 4 + st * 3 * NS / 8, NS / 4 + (st + 1) * 3 * NS / 8, acc);
             u32x4 hi, lo;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -632,31 +668,36 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
                     sum[j] += bf16lo(hi[j]) + bf16hi(hi[j]);
                 }
             }
-            p[0][st] = __builtin_bit_cast(bf16x8, hi);
-            if constexpr (kF32) p[1][st] = __builtin_bit_cast(bf16x8, lo);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const bf16x8 a = v_operand<NT>(v, t);
+                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, hi), o[t], 0, 0, 0);
+                if constexpr (kF32) {
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, lo), o[t], 0, 0, 0);
+                }
+            }
         }
         l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        const uint32_t vbase = (uint32_t)(uintptr_t)(lds_byte *)buf;
-#pragma unroll
-        for (int tg = 0; tg < NT / TPG; ++tg) {
-            uint32_t a[TPG];
-#pragma unroll
-            for (int t = 0; t < TPG; ++t) a[t] = vbase + v_at[tg * TPG + t];
-            VFrag<TPG> f;
-            read_v<D, 0>(f, a);
-#pragma unroll
-            for (int t = 0; t < TPG; ++t)
-#pragma unroll
-                for (int pp = 0; pp < T::PP; ++pp)
-                    o[tg * TPG + t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.get(t), p[pp][0], o[tg * TPG + t], 0, 0, 0);
-            VFrag<TPG> e;
-            read_v<D, 1>(e, a);
-#pragma unroll
-            for (int t = 0; t < TPG; ++t)
-#pragma unroll
-                for (int pp = 0; pp < T::PP; ++pp)
-                    o[tg * TPG + t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e.get(t), p[pp][1], o[tg * TPG + t], 0, 0, 0);
+        if constexpr (kNext) held = kChains == 2 ? acc[0] + acc[kChains - 1] : acc[0];
+    };
+    // steps + 1 barriers for every wave; stage k's scores run in step k, its softmax and
+    // P V in step k + 1
+    if (!live) {
+        for (uint32_t k = 0; k <= steps; ++k) enter(k);
+    } else {
+        enter(0);
+        {
+            f32x16 acc[kChains] = {};
+            scores(0, 0, NS, acc);
+            held = kChains == 2 ? acc[0] + acc[kChains - 1] : acc[0];
         }
+        for (uint32_t k = 1; k < steps; ++k) {
+            enter(k);
+            advance(k, std::true_type{});
+        }
+        enter(steps);
+        // (the last stage may end before the wave's keys)
+        if (key_begin + (steps - 1) * T::kKeys + 32 * kg < key_end) advance(steps, std::false_type{});
     }
     float l = half_sum(l_run);
     // join the waves over the keys, through the stages' LDS
@@ -698,34 +739,36 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
                                      tree_record_floats(D);
         if (h == 0) *(float2 *)rec = make_float2(m_run, l);
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int i = 0; i < 16; ++i) {
+            float *dst = rec + 4 + NT * (8 * (i >> 2) + 4 * h + (i & 3));
+            if constexpr (NT == 2) {
+                *(float2 *)dst = make_float2(o[0][i], o[1][i]);
+            } else {
 #pragma unroll
-            for (int a = 0; a < 4; ++a)
-                *(float4 *)(rec + 4 + 32 * t + 8 * a + 4 * h) =
-                    make_float4(o[t][4 * a], o[t][4 * a + 1], o[t][4 * a + 2], o[t][4 * a + 3]);
+                for (int t = 0; t < NT; t += 4) *(float4 *)(dst + t) = make_float4(o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]);
+            }
+        }
         return;
     }
     const bool gated = (c.flags & SAFETYRAISE_MI355X_GATED) != 0;
     const bool bf16_in = (c.flags & SAFETYRAISE_MI355X_INPUT_BF16) != 0;
+    const bool out16 = (c.flags & SAFETYRAISE_MI355X_OUTPUT_BF16) != 0;
     const float inv = 1.0f / l;
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t d = NT * (8 * (i >> 2) + 4 * h + (i & 3));
+        float y[NT];
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            const uint32_t d = 32 * t + 8 * a + 4 * h;
-            float y[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                y[j] = o[t][4 * a + j] * inv;
-                if (gated) y[j] *= ref_sigmoid(load_act(c.q, out_row * 2 * D + D + d + j, bf16_in));
-            }
-            if (c.flags & SAFETYRAISE_MI355X_OUTPUT_BF16) {
-                *(uint2 *)((uint16_t *)c.out + out_row * D + d) =
-                    make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
-            } else {
-                *(float4 *)((float *)c.out + out_row * D + d) = make_float4(y[0], y[1], y[2], y[3]);
-            }
+        for (int t = 0; t < NT; ++t) {
+            y[t] = o[t][i] * inv;
+            if (gated) y[t] *= ref_sigmoid(load_act(c.q, out_row * 2 * D + D + d + t, bf16_in));
         }
+#pragma unroll
+        for (int t = 0; t < NT; t += 2) {
+            if (out16) *(uint32_t *)((uint16_t *)c.out + out_row * D + d + t) = pack_bf16x2(y[t], y[t + 1]);
+            else *(float2 *)((float *)c.out + out_row * D + d + t) = make_float2(y[t], y[t + 1]);
+        }
+    }
 }
 
 // Joins the records of a (row, head): a wave each, all the loads of eight records
