@@ -231,8 +231,12 @@ int32_t commit(Ctx *ctx, const safetyraise_kernel_gdn_commit *commits, uint32_t 
     for (size_t i = 0; i < entries.size(); i += kMost) {
         const size_t count = std::min(kMost, entries.size() - i);
         if (count > kGdnCommitInline) {
-            const int32_t st = upload_words(ctx, (const uint32_t *)&entries[i],
-                                            count * sizeof(GdnCommitEntry) / 4, &device);
+            const size_t words = count * sizeof(GdnCommitEntry) / 4;
+            uint32_t *host = nullptr;
+            int32_t st = upload_room(ctx, words, &host);
+            if (st != kOk) return st;
+            std::memcpy(host, &entries[i], words * 4);
+            st = upload_words(ctx, words, &device);
             if (st != kOk) return st;
         } else {
             device = nullptr;

@@ -5,8 +5,8 @@
 // checked and planned before anything changes.
 
 #include <algorithm>
+#include <atomic>
 #include <cstring>
-#include <map>
 #include <utility>
 #include <vector>
 
@@ -16,9 +16,8 @@
 
 namespace sr {
 
-int32_t upload_words(Ctx *ctx, const uint32_t *words, size_t count, const uint32_t **out) {
+int32_t upload_room(Ctx *ctx, size_t count, uint32_t **host) {
     UploadSlot &u = ctx->upload[ctx->upload_next];
-    ctx->upload_next = (ctx->upload_next + 1) % kUploadSlots;
     const size_t bytes = (count * 4 + 15) & ~(size_t)15;
     if (u.pending) {
         SR_HIP(ctx, hipEventSynchronize(u.fetched));
@@ -36,11 +35,18 @@ int32_t upload_words(Ctx *ctx, const uint32_t *words, size_t count, const uint32
     }
     const int32_t st = ensure_buffer(ctx, u.dev, u.bytes, false);
     if (st != kOk) return st;
-    std::memcpy(u.host, words, count * 4);
-    SR_HIP(ctx, launch_linear_input(ctx->stream, (const float *)u.host_dev, (float *)u.dev.ptr, bytes / 4));
+    *host = (uint32_t *)u.host;
+    return kOk;
+}
+
+int32_t upload_words(Ctx *ctx, size_t count, const uint32_t **device) {
+    UploadSlot &u = ctx->upload[ctx->upload_next];
+    ctx->upload_next = (ctx->upload_next + 1) % kUploadSlots;
+    SR_HIP(ctx, launch_linear_input(ctx->stream, (const float *)u.host_dev, (float *)u.dev.ptr,
+                                    (count + 3) / 4 * 4));
     SR_HIP(ctx, hipEventRecord(u.fetched, ctx->stream));
     u.pending = true;
-    *out = (const uint32_t *)u.dev.ptr;
+    *device = (const uint32_t *)u.dev.ptr;
     return kOk;
 }
 
@@ -52,11 +58,63 @@ bool is_open(const Pool *pool, uint32_t seq) {
     return seq < pool->max_sequences && pool->seqs[seq].open;
 }
 
-template <class T>
-void put(std::vector<uint32_t> &words, const T &x) {
-    const size_t at = words.size();
-    words.resize(at + sizeof(T) / 4);
-    std::memcpy(words.data() + at, &x, sizeof(T));
+// The words of a call: in the kernel arguments (`small`) or in an upload slot.
+struct Words {
+    uint32_t small[kMoveInlineWords];
+    uint32_t *at = nullptr;
+
+    int32_t open(Ctx *ctx, size_t count, size_t most_inline) {
+        if (count <= most_inline) {
+            at = small;
+            return kOk;
+        }
+        return upload_room(ctx, count, &at);
+    }
+    // the device address, or nullptr for words in the arguments
+    int32_t send(Ctx *ctx, size_t count, const uint32_t **device) {
+        *device = nullptr;
+        return at == small ? kOk : upload_words(ctx, count, device);
+    }
+};
+
+// Token lists of a call by address: layers usually share them.
+struct Lists {
+    struct One {
+        const uint32_t *tokens;
+        uint64_t count;
+        uint32_t limit;  // all tokens are below it
+        bool ascending;
+        uint32_t offset;  // in the words; 0: not yet
+    };
+    std::vector<One> lists;
+
+    // the index of a list (a shared one may be there twice: only the last few are
+    // looked through)
+    uint32_t add(const uint32_t *tokens, uint64_t count) {
+        for (size_t i = lists.size(); i-- > 0 && i + 32 > lists.size();) {
+            if (lists[i].tokens == tokens && lists[i].count == count) return (uint32_t)i;
+        }
+        uint32_t most = 0;
+        bool ascending = true;
+        for (uint64_t j = 0; j < count; ++j) most = std::max(most, tokens[j]);
+        for (uint64_t j = 1; j < count; ++j) ascending &= tokens[j] > tokens[j - 1];
+        lists.push_back({tokens, count, count == 0 ? 0 : most + 1, ascending && most != UINT32_MAX, 0});
+        return (uint32_t)lists.size() - 1;
+    }
+};
+
+// A plan, and what it holds for (plans of other layers are often the same)
+struct KnownPlan {
+    const uint32_t *tokens;
+    uint64_t count, start;
+    uint32_t page_tokens;
+    bool in_place;
+    CompactPlan plan;
+};
+
+uint64_t next_call() {
+    static std::atomic<uint64_t> calls{0};
+    return ++calls;
 }
 
 int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n, uint32_t flags) {
@@ -64,38 +122,38 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
         return fail(ctx, kInvalid, "kv_compact needs entries, and no flag but ASYNC");
     }
     const bool async = (flags & SAFETYRAISE_MI355X_ASYNC) != 0;
-    // who is source and target of which entries
-    std::vector<std::pair<std::pair<Pool *, uint32_t>, uint32_t>> uses;  // (sequence, entry)
+    const uint64_t id = next_call();
+    Lists lists;
+    std::vector<uint32_t> list_of(n);
     for (uint32_t i = 0; i < n; ++i) {
         const auto &e = entries[i];
         if (e.kv == nullptr || !is_open(e.kv, e.source) || !is_open(e.kv, e.target)) {
             return fail(ctx, kInvalid, "KV sequence handle is not open");
         }
-        const uint64_t len = e.kv->seqs[e.source].len;
-        if (e.start > len || e.count > len - e.start || (e.count > 0 && e.tokens == nullptr)) {
+        auto &source = e.kv->seqs[e.source], &target = e.kv->seqs[e.target];
+        if (e.start > source.len || e.count > source.len - e.start || (e.count > 0 && e.tokens == nullptr)) {
             return fail(ctx, kInvalid, "KV token index out of range");
         }
-        for (uint64_t j = 0; j < e.count; ++j) {
-            if (e.tokens[j] >= len - e.start || (j > 0 && e.tokens[j] <= e.tokens[j - 1])) {
+        if (e.count > 0) {
+            list_of[i] = lists.add(e.tokens, e.count);
+            const Lists::One &l = lists.lists[list_of[i]];
+            if (!l.ascending || l.limit > source.len - e.start) {
                 return fail(ctx, kInvalid,
                             "kv_compact tokens must ascend strictly and stay within the sequence");
             }
         }
-        uses.push_back({{e.kv, e.source}, i});
-        if (e.target != e.source) uses.push_back({{e.kv, e.target}, i});
-    }
-    std::sort(uses.begin(), uses.end());
-    for (size_t i = 0; i < uses.size();) {
-        size_t end = i;
-        bool target = false;
-        while (end < uses.size() && uses[end].first == uses[i].first) {
-            target = target || entries[uses[end].second].target == uses[i].first.second;
-            ++end;
-        }
-        if (target && end - i > 1) {
+        if (target.source_of == id || target.target_of == id || source.target_of == id) {
             return fail(ctx, kInvalid, "a target of kv_compact may not appear in another entry");
         }
-        i = end;
+        source.source_of = id;
+        target.target_of = id;
+        if (e.kv->compact_call != id) {
+            e.kv->compact_call = id;
+            e.kv->compact_free = e.kv->free_pages.size();
+        }
+        if (e.target != e.source) {
+            for (int32_t page : target.pages) e.kv->compact_free += e.kv->refcount[page] == 1;
+        }
     }
     if (!async) {
         const int32_t st = report_pending_async(ctx);
@@ -103,43 +161,53 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
     }
 
     // plans, against the pages that are free now or that a target gives up
-    std::map<Pool *, uint64_t> free_pages;
-    for (uint32_t i = 0; i < n; ++i) {
-        Pool *pool = entries[i].kv;
-        auto at = free_pages.emplace(pool, pool->free_pages.size()).first;
-        if (entries[i].target == entries[i].source) continue;
-        for (int32_t page : pool->seqs[entries[i].target].pages) at->second += pool->refcount[page] == 1;
-    }
-    std::vector<CompactPlan> plans(n);
+    std::vector<KnownPlan> known;
+    std::vector<uint32_t> plan_of(n);
+    size_t ranges = 0, links = 0, words = 0;
+    uint32_t chains = 0, kv_heads = 1;
     for (uint32_t i = 0; i < n; ++i) {
         const auto &e = entries[i];
-        const auto &src = e.kv->seqs[e.source];
-        const KeepList keep{e.start, e.count, e.tokens};
-        uint64_t &free = free_pages[e.kv];
-        plans[i] = compact_plan(keep, e.kv->page_tokens, e.target == e.source, free, [&](uint64_t q) {
-            return e.kv->refcount[src.pages[q]] == 1;
-        });
-        if (plans[i].fresh > free) return fail(ctx, kNoMemory, "KV page pool exhausted");
-        free -= plans[i].fresh;
+        Pool *pool = e.kv;
+        const auto &old = pool->seqs[e.source].pages;
+        const bool in_place = e.target == e.source;
+        bool own = true;  // (of the pages that may be written)
+        const uint64_t pages = (e.start + e.count + pool->page_tokens - 1) / pool->page_tokens;
+        for (uint64_t q = e.start / pool->page_tokens; in_place && q < pages; ++q) own = own && pool->refcount[old[q]] == 1;
+        size_t at = known.size();
+        for (size_t k = known.size(); own && k-- > 0 && k + 16 > known.size();) {
+            const KnownPlan &x = known[k];
+            if (x.tokens == e.tokens && x.count == e.count && x.start == e.start &&
+                x.page_tokens == pool->page_tokens && x.in_place == in_place &&
+                x.plan.wanted <= pool->compact_free) {
+                at = k;
+                break;
+            }
+        }
+        if (at == known.size()) {
+            const KeepList keep{e.start, e.count, e.tokens};
+            known.push_back({own ? e.tokens : nullptr, own ? e.count : UINT64_MAX, e.start, pool->page_tokens, in_place,
+                             compact_plan(keep, pool->page_tokens, in_place, pool->compact_free,
+                                          [&](uint64_t q) { return pool->refcount[old[q]] == 1; })});
+        }
+        const CompactPlan &p = known[at].plan;
+        plan_of[i] = (uint32_t)at;
+        if (p.fresh > pool->compact_free) return fail(ctx, kNoMemory, "KV page pool exhausted");
+        pool->compact_free -= p.fresh;
+        ranges += p.ranges.size();
+        chains += (uint32_t)(p.serial ? std::min<size_t>(p.ranges.size(), 1) : p.ranges.size());
+        links += p.take.empty() ? 0 : 1;
+        words += p.take.size();
+        if (!p.ranges.empty()) kv_heads = std::max(kv_heads, pool->kv_heads);
     }
+    const size_t fixed = (n * sizeof(MoveEntry) + ranges * sizeof(MoveRange) + links * sizeof(MoveLink)) / 4;
+    words += fixed;
+    for (const Lists::One &l : lists.lists) words += l.count;
+    if (words > UINT32_MAX) return fail(ctx, kOverflow, "kv_compact is too large for one call");
+    Words w;
+    int32_t st = w.open(ctx, words, kMoveInlineWords);
+    if (st != kOk) return st;
 
-    // the new page lists, as the kernels' words
-    MoveCall call{};
-    std::vector<uint32_t> words, lists;
-    std::vector<MoveEntry> moves(n);
-    std::vector<MoveRange> heads, tails;
-    std::vector<MoveLink> links, late;
-    std::vector<std::vector<int32_t>> pages(n);
-    size_t ranges = 0;
-    for (const CompactPlan &p : plans) ranges += p.ranges.size();
-    size_t link_count = 0;
-    for (uint32_t i = 0; i < n; ++i) {
-        const uint64_t len = entries[i].start + entries[i].count;
-        link_count += len > plans[i].first * entries[i].kv->page_tokens ? 1 : 0;
-    }
-    const size_t fixed = (n * sizeof(MoveEntry) + ranges * sizeof(MoveRange) +
-                          (link_count + 1) * sizeof(MoveLink)) / 4;
-    // pages that targets give up first, so that they are free for the call
+    // nothing fails from here on but a launch: the new page lists, and the words
     for (uint32_t i = 0; i < n; ++i) {
         const auto &e = entries[i];
         if (e.target == e.source) continue;
@@ -148,104 +216,96 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
             if (--e.kv->refcount[page] == 0) e.kv->free_pages.push_back(page);
         }
         t.pages.clear();
-        t.len = 0;
     }
-    std::map<std::pair<const uint32_t *, uint64_t>, uint32_t> shared;  // token lists already there
-    for (uint32_t i = 0; i < n; ++i) {
+    MoveEntry *move = (MoveEntry *)w.at;
+    MoveRange *head = (MoveRange *)(move + n), *tail = head + chains;
+    MoveRange *const first_range = head;
+    MoveLink *link = (MoveLink *)(head + ranges);
+    std::vector<MoveLink> late;
+    std::vector<std::pair<Pool *, int32_t>> given_up;
+    uint32_t *list = w.at + fixed;
+    std::vector<int32_t> now;
+    MoveCall call{};
+    for (uint32_t i = 0; i < n; ++i, ++move) {
         const auto &e = entries[i];
         Pool *pool = e.kv;
-        const CompactPlan &p = plans[i];
-        const auto &old = pool->seqs[e.source].pages;
-        std::vector<int32_t> &now = pages[i];
-        now.assign(old.begin(), old.begin() + (ptrdiff_t)p.first);
-        for (int64_t take : p.take) {
-            if (take >= 0) {
-                now.push_back(old[(size_t)take]);
+        const CompactPlan &p = known[plan_of[i]].plan;
+        auto &source = pool->seqs[e.source], &target = pool->seqs[e.target];
+        const bool in_place = e.target == e.source;
+        bool changed = !in_place;
+        now.clear();
+        for (size_t q = 0; q < p.take.size(); ++q) {
+            int32_t page;
+            if (p.take[q] >= 0) {
+                page = source.pages[(size_t)p.take[q]];
+                ++pool->refcount[page];
+                changed = changed || (uint64_t)p.take[q] != p.first + q;
             } else {
-                now.push_back(pool->free_pages.back());
+                page = pool->free_pages.back();
                 pool->free_pages.pop_back();
-                pool->refcount[now.back()] = 0;
+                pool->refcount[page] = 1;
+                changed = true;
             }
+            now.push_back(page);
         }
-        for (int32_t page : now) ++pool->refcount[page];
-        MoveEntry &m = moves[i];
-        m.k_pages = pool->k_pages;
-        m.v_pages = pool->v_pages;
-        m.from = pool->d_page_table + (size_t)e.source * pool->pages_per_seq;
-        m.num_pages = pool->num_pages;
-        m.kv_heads = pool->kv_heads;
-        m.head_dim = pool->head_dim;
-        m.log2_page = (uint32_t)__builtin_ctz(pool->page_tokens);
-        m.start = (uint32_t)e.start;
-        m.first_page = (uint32_t)p.first;
-        m.pages = (uint32_t)(fixed + lists.size());
-        for (size_t q = p.first; q < now.size(); ++q) lists.push_back((uint32_t)now[q]);
-        if (!p.ranges.empty()) {
-            // layers usually keep the same tokens
-            const auto known = shared.emplace(std::make_pair(e.tokens, e.count), (uint32_t)(fixed + lists.size()));
-            if (known.second) lists.insert(lists.end(), e.tokens, e.tokens + e.count);
-            m.tokens = known.first->second;
-            call.kv_heads = std::max(call.kv_heads, pool->kv_heads);
+        *move = MoveEntry{};
+        move->k_pages = pool->k_pages;
+        move->v_pages = pool->v_pages;
+        move->from = pool->d_page_table + (size_t)e.source * pool->pages_per_seq;
+        move->num_pages = pool->num_pages;
+        move->kv_heads = pool->kv_heads;
+        move->head_dim = pool->head_dim;
+        move->log2_page = (uint32_t)__builtin_ctz(pool->page_tokens);
+        move->start = (uint32_t)e.start;
+        move->first_page = (uint32_t)p.first;
+        move->pages = (uint32_t)(list - w.at);
+        std::memcpy(list, now.data(), now.size() * 4);
+        list += now.size();
+        if (!p.ranges.empty() && e.count > 0) {
+            Lists::One &l = lists.lists[list_of[i]];
+            if (l.offset == 0) {
+                l.offset = (uint32_t)(list - w.at);
+                std::memcpy(list, e.tokens, e.count * 4);
+                list += e.count;
+            }
+            move->tokens = l.offset;
         }
-        bool changed = e.target != e.source;
-        for (size_t q = p.first; q < now.size() && !changed; ++q) changed = now[q] != old[q];
-        if (changed && now.size() > p.first) {
+        if (changed && !now.empty()) {
             const MoveLink l{pool->d_page_table + (size_t)e.target * pool->pages_per_seq + p.first,
-                             m.pages, (uint32_t)(now.size() - p.first)};
-            (e.target != e.source ? links : late).push_back(l);
+                             move->pages, (uint32_t)now.size()};
+            if (in_place) late.push_back(l);
+            else *link++ = l, ++call.links;
         }
+        MoveRange *last = nullptr;
         for (size_t r = 0; r < p.ranges.size(); ++r) {
-            const MoveRange range{i, (uint32_t)p.ranges[r].begin, (uint32_t)p.ranges[r].end, 0};
-            (p.serial && r > 0 ? tails : heads).push_back(range);
+            MoveRange *to = p.serial && r > 0 ? tail++ : head++;
+            *to = MoveRange{i, (uint32_t)p.ranges[r].begin, (uint32_t)p.ranges[r].end, 0};
+            if (p.serial && last != nullptr) last->next = (uint32_t)(to - first_range);
+            last = to;
         }
+        // the old pages from the first changed one on are given up, but not to this
+        // call's other entries: its ranges read them
+        if (in_place) {
+            for (size_t q = p.first; q < source.pages.size(); ++q) given_up.emplace_back(pool, source.pages[q]);
+            source.pages.resize(p.first);
+        }
+        target.pages.insert(target.pages.end(), now.begin(), now.end());
+        target.len = e.start + e.count;
     }
-    // chains: a serial entry's later ranges follow its first
-    {
-        size_t at = 0, head = 0;
-        for (uint32_t i = 0; i < n; ++i) {
-            const size_t count = plans[i].ranges.size();
-            if (plans[i].serial && count > 1) {
-                MoveRange *last = &heads[head];
-                for (size_t r = 1; r < count; ++r) {
-                    last->next = (uint32_t)(heads.size() + at);
-                    last = &tails[at++];
-                }
-            }
-            head += plans[i].serial ? std::min<size_t>(count, 1) : count;
-        }
+    for (const MoveLink &l : late) *link++ = l;
+    for (const auto &[pool, page] : given_up) {
+        if (--pool->refcount[page] == 0) pool->free_pages.push_back(page);
     }
     call.entries = n;
-    call.chains = (uint32_t)heads.size();
-    call.ranges = (uint32_t)(heads.size() + tails.size());
-    call.links = (uint32_t)links.size();
+    call.chains = chains;
+    call.ranges = (uint32_t)ranges;
     call.late_links = (uint32_t)late.size();
-    if (call.kv_heads == 0) call.kv_heads = 1;
-    for (const MoveEntry &m : moves) put(words, m);
-    for (const MoveRange &r : heads) put(words, r);
-    for (const MoveRange &r : tails) put(words, r);
-    for (const MoveLink &l : links) put(words, l);
-    for (const MoveLink &l : late) put(words, l);
-    words.resize(fixed);
-    words.insert(words.end(), lists.begin(), lists.end());
-    // the sequences have their new pages from here on, whatever the launches say
-    for (uint32_t i = 0; i < n; ++i) {
-        const auto &e = entries[i];
-        auto &t = e.kv->seqs[e.target];
-        if (e.target == e.source) {
-            for (int32_t page : t.pages) {
-                if (--e.kv->refcount[page] == 0) e.kv->free_pages.push_back(page);
-            }
-        }
-        t.pages = std::move(pages[i]);
-        t.len = e.start + e.count;
-    }
-    call.host_words = words.data();
-    call.words = (uint32_t)words.size();
+    call.kv_heads = kv_heads;
+    call.host_words = w.at;
+    call.words = (uint32_t)(list - w.at);
     if (call.chains + call.links + call.late_links > 0) {
-        if (words.size() > kMoveInlineWords) {
-            const int32_t st = upload_words(ctx, words.data(), words.size(), &call.device_words);
-            if (st != kOk) return st;
-        }
+        st = w.send(ctx, call.words, &call.device_words);
+        if (st != kOk) return st;
         SR_HIP(ctx, launch_kv_moves(ctx->stream, call));
     }
     return finish_call(ctx, async);
@@ -263,6 +323,8 @@ int32_t gather(Ctx *ctx, const safetyraise_kernel_kv_rows *entries, uint32_t n, 
     }
     if (async && !device) return fail(ctx, kInvalid, "ASYNC needs DEVICE_POINTERS");
     uint64_t total = 0;
+    Lists lists;
+    std::vector<uint32_t> list_of(n);
     for (uint32_t i = 0; i < n; ++i) {
         const auto &e = entries[i];
         if (e.kv == nullptr || !is_open(e.kv, e.sequence) || e.reserved != 0) {
@@ -271,14 +333,15 @@ int32_t gather(Ctx *ctx, const safetyraise_kernel_kv_rows *entries, uint32_t n, 
         if (e.kv->kv_heads != entries[0].kv->kv_heads || e.kv->head_dim != entries[0].kv->head_dim) {
             return fail(ctx, kInvalid, "kv_gather pools differ in kv_heads or head_dim");
         }
-        const uint64_t len = e.kv->seqs[e.sequence].len;
-        if (e.start > len || (e.tokens == nullptr && e.count > len - e.start)) {
-            return fail(ctx, kInvalid, "KV token index out of range");
-        }
-        for (uint64_t j = 0; e.tokens != nullptr && j < e.count; ++j) {
-            if (e.tokens[j] >= len - e.start) return fail(ctx, kInvalid, "KV token index out of range");
-        }
         if (e.count > INT32_MAX) return fail(ctx, kOverflow, "too many tokens");
+        const uint64_t len = e.kv->seqs[e.sequence].len;
+        bool inside = e.start <= len && (e.tokens != nullptr || e.count <= len - e.start);
+        if (inside && e.tokens != nullptr && e.count > 0) {
+            list_of[i] = lists.add(e.tokens, e.count);
+            const uint64_t limit = lists.lists[list_of[i]].limit;
+            inside = limit != 0 && limit <= len - e.start;  // (0: a token of 2^32 - 1)
+        }
+        if (!inside) return fail(ctx, kInvalid, "KV token index out of range");
         total += e.count;
     }
     if (!async) {
@@ -293,49 +356,65 @@ int32_t gather(Ctx *ctx, const safetyraise_kernel_kv_rows *entries, uint32_t n, 
     GatherCall call{};
     call.kv_heads = entries[0].kv->kv_heads;
     call.head_dim = entries[0].kv->head_dim;
-    call.tokens = total;
     call.bf16_out = out16;
     uint64_t bytes = 0;
     if (!checked_mul(total, (uint64_t)call.kv_heads * call.head_dim * (out16 ? 2 : 4), &bytes)) {
         return fail(ctx, kOverflow, "kv_gather size overflows");
     }
-    std::vector<uint32_t> words, lists;
-    std::map<std::pair<const uint32_t *, uint64_t>, uint32_t> shared;
-    const size_t fixed = n * sizeof(GatherEntry) / 4;
-    uint64_t first = 0;
+    // tokens of a workgroup: about 1024 of its threads' units
+    const uint64_t per = (uint64_t)call.kv_heads * (call.head_dim % 8 == 0 ? call.head_dim / 8 : call.head_dim);
+    call.block_tokens = (uint32_t)std::max<uint64_t>(1, 1024 / per);
+    uint64_t blocks = 0;
     for (uint32_t i = 0; i < n; ++i) {
+        call.entries += entries[i].count > 0;
+        blocks += (entries[i].count + call.block_tokens - 1) / call.block_tokens;
+    }
+    uint64_t words = (call.entries * sizeof(GatherEntry) + blocks * sizeof(GatherBlock)) / 4;
+    for (const Lists::One &l : lists.lists) words += l.count;
+    if (words > UINT32_MAX || blocks > INT32_MAX) return fail(ctx, kOverflow, "kv_gather is too large for one call");
+    Words w;
+    int32_t st = w.open(ctx, words, kGatherInlineWords);
+    if (st != kOk) return st;
+    GatherEntry *g = (GatherEntry *)w.at;
+    GatherBlock *block = (GatherBlock *)(g + call.entries);
+    uint32_t *list = (uint32_t *)(block + blocks);
+    uint64_t first = 0;
+    for (uint32_t i = 0, k = 0; i < n; ++i) {
         const auto &e = entries[i];
-        if (e.count == 0) continue;  // no token searches for it
-        GatherEntry g{};
-        g.k_pages = e.kv->k_pages;
-        g.v_pages = e.kv->v_pages;
-        g.from = e.kv->d_page_table + (size_t)e.sequence * e.kv->pages_per_seq;
-        g.num_pages = e.kv->num_pages;
-        g.first = first;
-        g.log2_page = (uint32_t)__builtin_ctz(e.kv->page_tokens);
-        g.start = (uint32_t)e.start;
+        if (e.count == 0) continue;
+        *g = GatherEntry{};
+        g->k_pages = e.kv->k_pages;
+        g->v_pages = e.kv->v_pages;
+        g->from = e.kv->d_page_table + (size_t)e.sequence * e.kv->pages_per_seq;
+        g->num_pages = (uint32_t)e.kv->num_pages;
+        g->first = first;
+        g->log2_page = (uint32_t)__builtin_ctz(e.kv->page_tokens);
+        g->start = (uint32_t)e.start;
+        g->count = (uint32_t)e.count;
         if (e.tokens != nullptr) {
-            const auto known = shared.emplace(std::make_pair(e.tokens, e.count), (uint32_t)(fixed + lists.size()));
-            if (known.second) lists.insert(lists.end(), e.tokens, e.tokens + e.count);
-            g.tokens = known.first->second;
+            Lists::One &l = lists.lists[list_of[i]];
+            if (l.offset == 0) {
+                l.offset = (uint32_t)(list - w.at);
+                std::memcpy(list, e.tokens, e.count * 4);
+                list += e.count;
+            }
+            g->tokens = l.offset;
         }
-        put(words, g);
-        ++call.entries;
+        for (uint64_t t = 0; t < e.count; t += call.block_tokens) *block++ = GatherBlock{k, (uint32_t)t};
         first += e.count;
+        ++g;
+        ++k;
     }
-    words.resize(fixed);
-    words.insert(words.end(), lists.begin(), lists.end());
-    call.host_words = words.data();
-    call.words = (uint32_t)words.size();
-    if (words.size() > kMoveInlineWords - 16) {
-        const int32_t st = upload_words(ctx, words.data(), words.size(), &call.device_words);
-        if (st != kOk) return st;
-    }
+    call.blocks = (uint32_t)blocks;
+    call.host_words = w.at;
+    call.words = (uint32_t)(list - w.at);
+    st = w.send(ctx, call.words, &call.device_words);
+    if (st != kOk) return st;
     call.keys = keys;
     call.values = values;
     const size_t half = (bytes + 255) & ~(size_t)255;
     if (!device) {
-        const int32_t st = ensure_buffer(ctx, ctx->staging, 2 * half, false);
+        st = ensure_buffer(ctx, ctx->staging, 2 * half, false);
         if (st != kOk) return st;
         call.keys = ctx->staging.ptr;
         call.values = (char *)ctx->staging.ptr + half;

@@ -12,6 +12,8 @@ namespace sr {
 
 namespace {
 
+typedef uint32_t Unit16 __attribute__((ext_vector_type(4)));  // 8 values
+
 struct MoveArgs {
     const uint32_t *words;  // nullptr: inline_words
     uint32_t entries, ranges, chains, links;
@@ -20,33 +22,45 @@ struct MoveArgs {
 static_assert(sizeof(MoveArgs) <= 4096, "kernel arguments stay within 4 KiB");
 
 // A workgroup moves the tokens of one range of one head's K or V, in the order
-// of the tokens: a chunk is read whole before any of it is written.
-template <typename Unit, uint32_t kUnits>
+// of the tokens: a chunk is read whole before any of it is written.  A row is `per`
+// units; a thread has one of them in every pass of 256 / per rows (rows of more than
+// 256 units: 256 / per is 0, and a thread takes every 256th unit of one row).
+template <typename Unit, uint32_t kPasses>
 __device__ __forceinline__ void move_range(uint16_t *pages, const MoveEntry &e, const MoveRange &r,
                                            const int32_t *from, const int32_t *to,
                                            const uint32_t *tokens, uint32_t kvh) {
-    const uint32_t per = (uint32_t)(e.head_dim * 2 / sizeof(Unit));  // units per row
+    const uint32_t per = (uint32_t)(e.head_dim * 2 / sizeof(Unit));  // at most 512 units
     const uint32_t lpt = e.log2_page, mask = (1u << lpt) - 1;
-    Unit *base = (Unit *)(pages + (((size_t)kvh * e.num_pages) << lpt) * e.head_dim);
-    const uint64_t total = (uint64_t)(r.end - r.begin) * per;
-    for (uint64_t u0 = 0; u0 < total; u0 += 256 * kUnits) {
-        Unit x[kUnits];
-        size_t dst[kUnits];
+    Unit *base = global_from_bits<Unit>((uint64_t)(pages + (((size_t)kvh * e.num_pages) << lpt) * e.head_dim));
+    const uint32_t rows = per <= 256 ? 256 / per : 1;  // of a pass
+    const uint32_t my_row = per <= 256 ? threadIdx.x / per : 0;
+    const uint32_t my_unit = per <= 256 ? threadIdx.x % per : threadIdx.x;
+    for (uint32_t t0 = r.begin; t0 < r.end; t0 += rows * kPasses) {
+        for (uint32_t u0 = 0; u0 < per; u0 += 256) {  // (once, but for rows of more than 256 units)
+            const uint32_t u = min(u0 + my_unit, per - 1);
+            Unit x[kPasses];
+            Unit *dst[kPasses];
+            bool ok[kPasses];
+            uint32_t s[kPasses];
 #pragma unroll
-        for (uint32_t i = 0; i < kUnits; ++i) {
-            const uint64_t u = min(u0 + threadIdx.x + 256 * i, total - 1);
-            const uint32_t t = r.begin + (uint32_t)(u / per), at = (uint32_t)(u % per);
-            const uint32_t s = t < e.start ? t : e.start + tokens[t - e.start];
-            const int32_t src_page = from[s >> lpt], dst_page = to[(t >> lpt) - e.first_page];
-            x[i] = base[(((size_t)src_page << lpt) + (s & mask)) * per + at];
-            dst[i] = (((size_t)dst_page << lpt) + (t & mask)) * per + at;
-        }
-        // every wave's reads are done before any wave writes
-        __builtin_amdgcn_s_waitcnt(0x0F70);
-        __syncthreads();
+            for (uint32_t i = 0; i < kPasses; ++i) {
+                const uint32_t t = t0 + rows * i + my_row;
+                ok[i] = my_row < rows && u0 + my_unit < per && t < r.end;
+                const uint32_t tc = ok[i] ? t : r.begin;
+                s[i] = tc < e.start ? tc : e.start + tokens[tc - e.start];
+                dst[i] = base + (((size_t)to[(tc >> lpt) - e.first_page] << lpt) + (tc & mask)) * per + u;
+            }
 #pragma unroll
-        for (uint32_t i = 0; i < kUnits; ++i) {
-            if (u0 + threadIdx.x + 256 * i < total) base[dst[i]] = x[i];
+            for (uint32_t i = 0; i < kPasses; ++i) {
+                x[i] = base[(((size_t)from[s[i] >> lpt] << lpt) + (s[i] & mask)) * per + u];
+            }
+            // every wave's reads are done before any wave writes
+            __builtin_amdgcn_s_waitcnt(0x0F70);
+            __syncthreads();
+#pragma unroll
+            for (uint32_t i = 0; i < kPasses; ++i) {
+                if (ok[i]) *dst[i] = x[i];
+            }
         }
     }
 }
@@ -65,14 +79,15 @@ __global__ void __launch_bounds__(256) kv_move_kernel(const MoveArgs a) {
     }
     MoveRange r = ranges[blockIdx.x];
     const MoveEntry e = entries[r.entry];
+    const int32_t *from = global_from_bits<const int32_t>((uint64_t)e.from);
     const uint32_t kvh = blockIdx.y >> 1;
     if (kvh >= e.kv_heads) return;
     uint16_t *pages = (blockIdx.y & 1) ? e.v_pages : e.k_pages;
     const int32_t *to = (const int32_t *)(w + e.pages);
     const uint32_t *tokens = w + e.tokens;
     for (;;) {
-        if (e.head_dim % 8 == 0) move_range<uint4, 4>(pages, e, r, e.from, to, tokens, kvh);
-        else move_range<uint16_t, 8>(pages, e, r, e.from, to, tokens, kvh);
+        if (e.head_dim % 8 == 0) move_range<Unit16, 4>(pages, e, r, from, to, tokens, kvh);
+        else move_range<uint16_t, 4>(pages, e, r, from, to, tokens, kvh);
         if (r.next == 0) break;
         r = ranges[r.next];
     }
@@ -88,56 +103,73 @@ struct GatherArgs {
     const uint32_t *words;
     void *keys;
     void *values;
-    uint64_t tokens;
-    uint32_t entries, kv_heads, head_dim;
+    uint32_t entries, kv_heads, head_dim, block_tokens;
     int bf16_out;
-    alignas(16) uint32_t inline_words[kMoveInlineWords - 16];
+    alignas(16) uint32_t inline_words[kGatherInlineWords];
 };
 static_assert(sizeof(GatherArgs) <= 4096, "kernel arguments stay within 4 KiB");
 
-// One thread per 8 values (kVec) or one value of a token's K and V rows.
+// One workgroup per block of at most block_tokens tokens of one entry; a thread
+// takes 8 values (kVec) or one value of a token's K and V rows at a time.
 template <bool kVec>
 __global__ void __launch_bounds__(256) kv_gather_rows_kernel(const GatherArgs a) {
     const uint32_t *w = a.words != nullptr ? a.words : a.inline_words;
     const GatherEntry *entries = (const GatherEntry *)w;
+    const GatherBlock b = ((const GatherBlock *)(entries + a.entries))[blockIdx.x];
+    const GatherEntry e = entries[b.entry];
+    const uint16_t *k_pages = global_from_bits<const uint16_t>((uint64_t)e.k_pages);
+    const uint16_t *v_pages = global_from_bits<const uint16_t>((uint64_t)e.v_pages);
+    const int32_t *from = global_from_bits<const int32_t>((uint64_t)e.from);
     const uint32_t per_head = kVec ? a.head_dim / 8 : a.head_dim;
     const uint32_t per = a.kv_heads * per_head;
-    const uint64_t n = a.tokens * per;
-    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += (uint64_t)gridDim.x * 256) {
-        const uint64_t t = i / per;
-        const uint32_t r = (uint32_t)(i % per), h = r / per_head, c = r % per_head;
-        uint32_t lo = 0, hi = a.entries - 1;  // the entry that holds token t
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi + 1) / 2;
-            if (entries[mid].first <= t) lo = mid;
-            else hi = mid - 1;
+    const uint32_t n = min(a.block_tokens, e.count - b.begin) * per;
+    constexpr uint32_t kBatch = 4;
+    for (uint32_t i0 = threadIdx.x; i0 < n; i0 += 256 * kBatch) {
+        size_t src[kBatch], dst[kBatch];
+        bool ok[kBatch];
+#pragma unroll
+        for (uint32_t u = 0; u < kBatch; ++u) {
+            ok[u] = i0 + 256 * u < n;
+            const uint32_t i = ok[u] ? i0 + 256 * u : i0;
+            const uint32_t at = b.begin + i / per, r = i % per, h = r / per_head, c = r % per_head;
+            const uint32_t s = e.start + (e.tokens != 0 ? w[e.tokens + at] : at);
+            const size_t row = (((size_t)h * e.num_pages + from[s >> e.log2_page]) << e.log2_page) +
+                               (s & ((1u << e.log2_page) - 1));
+            src[u] = row * a.head_dim + (kVec ? 8 * c : c);
+            dst[u] = (e.first + at) * per + r;
         }
-        const GatherEntry e = entries[lo];
-        const uint32_t at = (uint32_t)(t - e.first);
-        const uint32_t s = e.start + (e.tokens != 0 ? w[e.tokens + at] : at);
-        const size_t row = (((size_t)h * e.num_pages + e.from[s >> e.log2_page]) << e.log2_page) +
-                           (s & ((1u << e.log2_page) - 1));
         if constexpr (kVec) {
-            const size_t src = row * a.head_dim + 8 * c;
-            const uint4 k = *(const uint4 *)(e.k_pages + src), v = *(const uint4 *)(e.v_pages + src);
-            if (a.bf16_out) {
-                ((uint4 *)a.keys)[i] = k;
-                ((uint4 *)a.values)[i] = v;
-            } else {
-                float4 *dk = (float4 *)a.keys + 2 * i, *dv = (float4 *)a.values + 2 * i;
-                dk[0] = make_float4(bf16lo(k.x), bf16hi(k.x), bf16lo(k.y), bf16hi(k.y));
-                dk[1] = make_float4(bf16lo(k.z), bf16hi(k.z), bf16lo(k.w), bf16hi(k.w));
-                dv[0] = make_float4(bf16lo(v.x), bf16hi(v.x), bf16lo(v.y), bf16hi(v.y));
-                dv[1] = make_float4(bf16lo(v.z), bf16hi(v.z), bf16lo(v.w), bf16hi(v.w));
+            Unit16 k[kBatch], v[kBatch];
+#pragma unroll
+            for (uint32_t u = 0; u < kBatch; ++u) {
+                k[u] = *(const Unit16 *)(k_pages + src[u]);
+                v[u] = *(const Unit16 *)(v_pages + src[u]);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < kBatch; ++u) {
+                if (!ok[u]) break;
+                if (a.bf16_out) {
+                    ((Unit16 *)a.keys)[dst[u]] = k[u];
+                    ((Unit16 *)a.values)[dst[u]] = v[u];
+                } else {
+                    float4 *dk = (float4 *)a.keys + 2 * dst[u], *dv = (float4 *)a.values + 2 * dst[u];
+                    dk[0] = make_float4(bf16lo(k[u].x), bf16hi(k[u].x), bf16lo(k[u].y), bf16hi(k[u].y));
+                    dk[1] = make_float4(bf16lo(k[u].z), bf16hi(k[u].z), bf16lo(k[u].w), bf16hi(k[u].w));
+                    dv[0] = make_float4(bf16lo(v[u].x), bf16hi(v[u].x), bf16lo(v[u].y), bf16hi(v[u].y));
+                    dv[1] = make_float4(bf16lo(v[u].z), bf16hi(v[u].z), bf16lo(v[u].w), bf16hi(v[u].w));
+                }
             }
         } else {
-            const size_t src = row * a.head_dim + c;
-            if (a.bf16_out) {
-                ((uint16_t *)a.keys)[i] = e.k_pages[src];
-                ((uint16_t *)a.values)[i] = e.v_pages[src];
-            } else {
-                ((float *)a.keys)[i] = bf16_to_f32(e.k_pages[src]);
-                ((float *)a.values)[i] = bf16_to_f32(e.v_pages[src]);
+#pragma unroll
+            for (uint32_t u = 0; u < kBatch; ++u) {
+                if (!ok[u]) break;
+                if (a.bf16_out) {
+                    ((uint16_t *)a.keys)[dst[u]] = k_pages[src[u]];
+                    ((uint16_t *)a.values)[dst[u]] = v_pages[src[u]];
+                } else {
+                    ((float *)a.keys)[dst[u]] = bf16_to_f32(k_pages[src[u]]);
+                    ((float *)a.values)[dst[u]] = bf16_to_f32(v_pages[src[u]]);
+                }
             }
         }
     }
@@ -174,20 +206,20 @@ hipError_t launch_kv_gather_rows(hipStream_t stream, const GatherCall &c) {
     a.words = c.device_words;
     a.keys = c.keys;
     a.values = c.values;
-    a.tokens = c.tokens;
     a.entries = c.entries;
     a.kv_heads = c.kv_heads;
     a.head_dim = c.head_dim;
+    a.block_tokens = c.block_tokens;
     a.bf16_out = c.bf16_out ? 1 : 0;
     if (a.words == nullptr) {
-        if (c.words > kMoveInlineWords - 16) return hipErrorInvalidValue;
+        if (c.words > kGatherInlineWords) return hipErrorInvalidValue;
         for (uint32_t i = 0; i < c.words; ++i) a.inline_words[i] = c.host_words[i];
     }
-    const bool vec = c.head_dim % 8 == 0;
-    const uint64_t n = c.tokens * c.kv_heads * (vec ? c.head_dim / 8 : c.head_dim);
-    const uint32_t blocks = (uint32_t)std::min<uint64_t>((n + 255) / 256, 65536);
-    if (vec) SR_LAUNCH("kv_gather_rows_kernel", kv_gather_rows_kernel<true>, dim3(blocks), dim3(256), 0, stream, a);
-    else SR_LAUNCH("kv_gather_rows_kernel", kv_gather_rows_kernel<false>, dim3(blocks), dim3(256), 0, stream, a);
+    if (c.head_dim % 8 == 0) {
+        SR_LAUNCH("kv_gather_rows_kernel", kv_gather_rows_kernel<true>, dim3(c.blocks), dim3(256), 0, stream, a);
+    } else {
+        SR_LAUNCH("kv_gather_rows_kernel", kv_gather_rows_kernel<false>, dim3(c.blocks), dim3(256), 0, stream, a);
+    }
     return hipGetLastError();
 }
 

@@ -34,17 +34,21 @@ struct GatherEntry {
     const uint16_t *k_pages;
     const uint16_t *v_pages;
     const int32_t *from;
-    uint64_t num_pages;
     uint64_t first;  // the entry's first token in the output
-    uint32_t log2_page, start;
+    uint32_t num_pages, log2_page, start, count;
     uint32_t tokens;  // 0: consecutive tokens
     uint32_t unused;
+};
+// a workgroup's tokens: block_tokens of the entry from `begin` on, as far as it has them
+struct GatherBlock {
+    uint32_t entry, begin;
 };
 static_assert(sizeof(MoveEntry) % 8 == 0 && sizeof(MoveRange) % 8 == 0 && sizeof(MoveLink) % 8 == 0 &&
                   sizeof(GatherEntry) % 8 == 0,
               "pointers stay aligned");
 
 constexpr uint32_t kMoveInlineWords = 1008;  // what fits the kernel arguments
+constexpr uint32_t kGatherInlineWords = 992;
 
 struct MoveCall {
     const uint32_t *host_words;
@@ -59,8 +63,7 @@ struct GatherCall {
     const uint32_t *host_words;
     const uint32_t *device_words;
     uint32_t words;
-    uint32_t entries, kv_heads, head_dim;
-    uint64_t tokens;
+    uint32_t entries, blocks, kv_heads, head_dim, block_tokens;
     void *keys, *values;
     bool bf16_out;
 };

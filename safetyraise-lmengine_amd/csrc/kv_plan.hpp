@@ -13,6 +13,9 @@ namespace sr {
 // page at once, as far as the pool has them.
 constexpr uint64_t kCompactSerial = 256;
 
+// Tokens that one workgroup copies where ranges run at once.
+constexpr uint64_t kCompactRange = 64;
+
 // One sequence's kept tokens: new token t is old token from(t).
 struct KeepList {
     uint64_t start, count;
@@ -27,6 +30,7 @@ struct CompactPlan {
     uint64_t first = 0;
     std::vector<int64_t> take;  // pages first, first + 1, ...
     uint64_t fresh = 0;         // free pages needed
+    uint64_t wanted = 0;        // free pages with which the plan would be the same
     // token ranges to copy; the ranges of a serial plan run in order in one
     // workgroup per head, others at once
     struct Range {
@@ -89,7 +93,9 @@ CompactPlan compact_plan(const KeepList &k, uint64_t page_tokens, bool into_sour
     }
     uint64_t least = 0;
     for (uint64_t q : copied) least += in_place(q) ? 0 : 1;
+    plan.wanted = fresh;
     plan.serial = into_source && least < fresh && (tokens <= kCompactSerial || fresh > free);
+    bool first_stays = false;
     for (uint64_t i = 0; i < copied.size(); ++i) {
         const uint64_t q = copied[i];
         const bool stay = in_place(q) && (plan.serial || (i == 0 && q == plan.first));
@@ -97,7 +103,16 @@ CompactPlan compact_plan(const KeepList &k, uint64_t page_tokens, bool into_sour
         else ++plan.fresh;
         // (tokens before the first moved one are in place already)
         const uint64_t begin = stay ? std::max(q * page_tokens, moved) : q * page_tokens;
-        if (begin < end_of(q)) plan.ranges.push_back({begin, end_of(q)});
+        if (begin >= end_of(q)) continue;
+        // pages in a row make one range: all of a serial plan's, else up to kCompactRange
+        // tokens, but for the page that is filled where it is
+        if (i > 0 && !plan.ranges.empty() && plan.ranges.back().end == begin &&
+            (plan.serial || (end_of(q) - plan.ranges.back().begin <= kCompactRange && !first_stays))) {
+            plan.ranges.back().end = end_of(q);
+        } else {
+            plan.ranges.push_back({begin, end_of(q)});
+        }
+        first_stays = stay && !plan.serial;
     }
     return plan;
 }

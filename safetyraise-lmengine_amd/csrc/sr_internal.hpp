@@ -172,8 +172,10 @@ struct safetyraise_kernel_kv_pool {
         bool open = false;
         uint64_t len = 0;
         std::vector<int32_t> pages;
+        uint64_t source_of = 0, target_of = 0;  // the kv_compact call that last named it so
     };
     std::vector<Sequence> seqs;
+    uint64_t compact_call = 0, compact_free = 0;  // free pages left to a kv_compact call's entries
     std::vector<uint32_t> refcount;
     std::vector<int32_t> free_pages;
     size_t page_elems() const { return (size_t)kv_heads * page_tokens * head_dim; }
@@ -303,9 +305,11 @@ int32_t kv_prepare_append(Ctx *ctx, safetyraise_kernel_kv_pool *pool, uint32_t s
                           TableBatch *batch = nullptr);
 int32_t kv_flush_table(Ctx *ctx, safetyraise_kernel_kv_pool *pool, TableBatch &batch);
 
-// `count` words of a call's description in device memory (*out), valid for work queued
-// on the context's stream after this.
-int32_t upload_words(Ctx *ctx, const uint32_t *words, size_t count, const uint32_t **out);
+// Room for `count` words of a call's description in pinned memory (*host), and their
+// way to the device: upload_words launches the copy and gives the device address,
+// valid for work queued on the context's stream after it.
+int32_t upload_room(Ctx *ctx, size_t count, uint32_t **host);
+int32_t upload_words(Ctx *ctx, size_t count, const uint32_t **device);
 
 // ---------------- kernel launchers (defined in the .hip files) ----------------
 hipError_t launch_page_table_set(hipStream_t s, int32_t *table, const uint32_t *idx,

@@ -76,6 +76,36 @@ def test_commit_in_place(backend, dim, page):
     m.pool.destroy()
 
 
+@pytest.mark.parametrize("dim", [257, 300, 511, 512])
+def test_wide_rows(backend, dim):
+    """Rows of more units than a workgroup has threads."""
+    rng = np.random.default_rng(dim)
+    m = Model(backend, rng, 2, dim, 16)
+    s, b, c = m.new(60), m.new(90), m.new(0)
+    compact(backend, [(m, s, s, 33, [1, 2, 7, 20]), (m, b, c, 10, list(range(0, 80, 3)))])
+    m.check()
+    k, v = (np.zeros((39, m.width), np.float32) for _ in range(2))
+    pkg.kv_gather(backend, [(m.pool, c, 5, [0, 7, 3]), (m.pool, s, 0, 36)], k, v)
+    at = [5, 12, 8]
+    for got, c_rows, s_rows in ((k, m.held[c][0], m.held[s][0]), (v, m.held[c][1], m.held[s][1])):
+        assert np.array_equal(got, np.concatenate([c_rows[at], s_rows[:36]]))
+    m.pool.destroy()
+
+
+def test_pages_given_up_are_still_read(backend):
+    """A page that one entry gives up is no free page to the entries behind it: the
+    call's copies still read it."""
+    rng = np.random.default_rng(11)
+    for page in (16, 64):
+        m = Model(backend, rng, 2, 64, page, pages=40)
+        a, b, c = m.new(5 * page - 1), m.new(4 * page), m.new(0)
+        tokens = [2 * page + 3, 3 * page + 1, 4 * page + 2]
+        compact(backend, [(m, a, a, page + 2, [t - page - 2 for t in tokens]),
+                          (m, b, c, 3, list(range(0, 4 * page - 3, 2)))])
+        m.check()
+        m.pool.destroy()
+
+
 @pytest.mark.parametrize("tokens", [[], [0], [19], list(range(20)), list(range(5)), list(range(16, 20)),
                                     list(range(4, 20))])
 def test_edges(backend, tokens):
