@@ -27,6 +27,7 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kTreeSeqs = kTreeLaunchSeqs;
@@ -54,8 +55,8 @@ struct TreeCommon {
     uint64_t num_pages;
     uint32_t pages_per_seq, log2_page;
     uint32_t flags, heads, kv_heads, head_dim;
-    uint32_t nseq, part_keys, vectors;  // vectors: query vectors per workgroup
-    TreeMeta meta[kTreeSeqs];
+    uint32_t nseq, part_keys;
+    alignas(16) TreeMeta meta[kTreeSeqs];
 };
 
 struct PrepParams {
@@ -73,18 +74,28 @@ struct PrepParams {
     uint32_t tbl_idx[kInlineTable];
     int32_t tbl_val[kInlineTable];
     float denom[kGenericMaxHeadDim / 2];
-    uint8_t parent[kTreeRows];  // parent + 1 within the sequence, 0 for a root
+    alignas(16) uint8_t parent[kTreeRows];  // parent + 1 within the sequence, 0 for a root
 };
 static_assert(sizeof(PrepParams) <= 4096, "kernel arguments stay within 4 KiB");
 
-constexpr uint32_t kPrepHeads = 4;  // heads of one row per wave
+constexpr uint32_t kPrepHeads = 1;  // heads of one row per wave
 constexpr uint32_t kPrepDims = kGenericMaxHeadDim / 64;
 
-// The sequence of launch row `r` (rows are numbered from the launch's first).
-__device__ __forceinline__ uint32_t find_row(const TreeCommon &c, uint32_t r) {
-    uint32_t s = 0;
-    while (s + 1 < c.nseq && c.meta[s + 1].row0 - c.meta[0].row0 <= r) ++s;
-    return s;
+// The sequence of launch row `r` (rows are numbered from the launch's first), or of
+// workgroup `r` of the attention kernel.  The arguments of a launch lie in memory far
+// away: a wave reads all the sequences' at once, half of one per lane, instead of one
+// after another.
+template <bool kBlock>
+__device__ __forceinline__ TreeMeta find_meta(const TreeCommon &c, uint32_t r) {
+    static_assert(kTreeSeqs == 32 && sizeof(TreeMeta) == 32, "two lanes per sequence");
+    const uint32_t lane = threadIdx.x & 63;
+    const u32x4 x = ((const u32x4 *)c.meta)[lane];  // {slot, ctx, rows, row0} | {tile0, block0, record0, parts}
+    const uint32_t begin = kBlock ? x.y : x.w - (uint32_t)__builtin_amdgcn_readfirstlane((int)x.w);
+    const bool before = (lane & 1) == (kBlock ? 1u : 0u) && lane / 2 < c.nseq && begin <= r;
+    const int at = 2 * (__popcll(__builtin_amdgcn_ballot_w64(before)) - 1);
+    auto get = [&](uint32_t v, int i) { return (uint32_t)__builtin_amdgcn_readlane((int)v, i); };
+    return TreeMeta{get(x.x, at), get(x.y, at), get(x.z, at), get(x.w, at),
+                    get(x.x, at + 1), get(x.y, at + 1), get(x.z, at + 1), get(x.w, at + 1)};
 }
 
 // One wave per (row, four heads): KV heads first, then query heads.  NI: dims
@@ -107,8 +118,16 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(const PrepParams p) {
     }
     if (item >= p.rows * groups) return;
     const uint32_t r = item / groups, h0 = item % groups * kPrepHeads;
-    const uint32_t s = find_row(c, r);
-    const TreeMeta m = c.meta[s];
+    // what the wave needs of the arguments' tables, a part per lane
+    constexpr uint32_t kPairs = (NI + 1) / 2;  // rotary pairs per lane
+    static_assert(kTreeRows == 64 * 16 && kInlineTable == 64, "a lane's part of the tables");
+    float denom[kPairs];
+#pragma unroll
+    for (uint32_t i = 0; i < kPairs; ++i) denom[i] = p.denom[lane + 64 * i];
+    const uint32_t tbl_idx = lane < p.tbl_n ? p.tbl_idx[lane] : ~0u;
+    const int32_t tbl_val = p.tbl_val[lane];
+    const u32x4 parents = ((const u32x4 *)p.parent)[lane];
+    const TreeMeta m = find_meta<false>(c, r);
     const uint32_t row = m.row0 + (r - (m.row0 - c.meta[0].row0));
     const uint32_t sr = row - m.row0;  // row of the sequence
     const bool bf16_in = (c.flags & SAFETYRAISE_MI355X_INPUT_BF16) != 0;
@@ -118,6 +137,12 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(const PrepParams p) {
     const bool interleaved = (c.flags & SAFETYRAISE_MI355X_MROPE_INTERLEAVED) != 0;
     const size_t hs = gated ? 2 * (size_t)D : D;
 
+    const int32_t *pos = p.positions + (size_t)row * 3;
+    const int32_t pos0 = pos[0], pos1 = pos[1], pos2 = pos[2];
+    // the row's page: its entry may be among those that this launch writes
+    const uint32_t tok = m.ctx + sr;
+    const uint32_t entry = m.slot * c.pages_per_seq + (tok >> c.log2_page);
+    int32_t page = c.page_table[entry];
     // all of the wave's values are requested before any is used
     float x[kPrepHeads][NI], v[kPrepHeads][NI];
 #pragma unroll
@@ -134,23 +159,38 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(const PrepParams p) {
             v[u][i] = kv ? load_act_nb(p.v, at + d, bf16_in) : 0.0f;
         }
     }
-    // the row's page: its entry may be among those that this launch writes
-    const uint32_t tok = m.ctx + sr;
-    const uint32_t entry = m.slot * c.pages_per_seq + (tok >> c.log2_page);
-    int32_t page = c.page_table[entry];
-    for (uint32_t i = 0; i < p.tbl_n; ++i) {
-        if (p.tbl_idx[i] == entry) page = p.tbl_val[i];
-    }
+    const uint64_t own = __builtin_amdgcn_ballot_w64(tbl_idx == entry);
+    if (own != 0) page = __builtin_amdgcn_readlane(tbl_val, __builtin_ctzll(own));
     if (h0 == 0) {
         // the ancestors, walked from the row to its root
         uint32_t w[4] = {0, 0, 0, 0};
-        const uint8_t *parent = p.parent + (m.row0 - c.meta[0].row0);
-        for (uint32_t a = sr + 1; a != 0; a = parent[a - 1]) {
+        const uint32_t first = m.row0 - c.meta[0].row0;
+        for (uint32_t a = sr + 1; a != 0;) {
             const uint32_t b = a - 1;
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) w[k] |= (b >> 5) == k ? 1u << (b & 31) : 0u;
+            const uint32_t at = first + b, word = at / 4 % 4;
+            uint32_t four = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) {
+                const uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)parents[k], (int)(at / 16));
+                four = word == k ? x : four;
+            }
+            a = (four >> (at % 4 * 8)) & 0xffu;
         }
         if (lane == 0) c.masks[row] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    // the rotation, while the values are on their way
+    const uint32_t half = p.rotary_dim / 2;
+    float sn[kPairs], cs[kPairs];
+#pragma unroll
+    for (uint32_t i = 0; i < kPairs; ++i) {
+        const int axis = rope_axis(lane + 64 * i, p.mrope, interleaved);
+        sn[i] = 0.0f;
+        cs[i] = 1.0f;
+        if (lane + 64 * i < half) {
+            sincosf((float)(axis == 0 ? pos0 : axis == 1 ? pos1 : pos2) / denom[i], &sn[i], &cs[i]);
+        }
     }
     if (norm) {
 #pragma unroll
@@ -183,17 +223,15 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(const PrepParams p) {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     // rotate-half over the first rotary_dim dims (math.rs:52-99)
-    const int32_t *pos = p.positions + (size_t)row * 3;
-    const uint32_t half = p.rotary_dim / 2;
-    for (uint32_t i = lane; i < half; i += 64) {
-        const int axis = rope_axis(i, p.mrope, interleaved);
-        float sn, cs;
-        sincosf((float)pos[axis] / p.denom[i], &sn, &cs);
+#pragma unroll
+    for (uint32_t k = 0; k < kPairs; ++k) {
+        const uint32_t i = lane + 64 * k;
+        if (i >= half) continue;
 #pragma unroll
         for (uint32_t u = 0; u < kPrepHeads; ++u) {
             const float left = xs[u * D + i], right = xs[u * D + i + half];
-            xs[u * D + i] = left * cs - right * sn;
-            xs[u * D + i + half] = right * cs + left * sn;
+            xs[u * D + i] = left * cs[k] - right * sn[k];
+            xs[u * D + i + half] = right * cs[k] + left * sn[k];
         }
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -281,8 +319,7 @@ __global__ void __launch_bounds__(64) tree_generic_kernel(const TreeCommon c) {
     const uint32_t D = c.head_dim, lane = threadIdx.x;
     float *qs = sh, *ps = sh + D;
     const uint32_t head = blockIdx.x, r = blockIdx.y;
-    const uint32_t s = find_row(c, r);
-    const TreeMeta m = c.meta[s];
+    const TreeMeta m = find_meta<false>(c, r);
     const uint32_t sr = r - (m.row0 - c.meta[0].row0);
     const size_t row = (size_t)m.row0 + sr;
     const float *q = (const float *)c.q_ops + ((size_t)r * c.heads + head) * D;
@@ -376,7 +413,7 @@ struct TreeShape {
     static constexpr int NW = VG * KG;
     static constexpr int kThreads = 64 * NW;
     static constexpr int QP = kF32 ? 3 : 2;     // bf16 parts of q
-    static constexpr int PP = kF32 ? 2 : 1;     // of the probabilities
+    static constexpr int PP = kF32 ? 3 : 1;     // of the probabilities
     static constexpr size_t kLds = kStages * kStageBytes + kTreePageSlots * 4;
 };
 
@@ -433,10 +470,10 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
 
     const uint32_t tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = (uint32_t)wave_index();
-    const uint32_t vg = wave % VG, kg = wave / VG;
-    uint32_t s = 0;
-    while (s + 1 < c.nseq && c.meta[s + 1].block0 <= blockIdx.x) ++s;
-    const TreeMeta m = c.meta[s];
+    // (wave i runs on SIMD i % 4: the waves of one vector group on different ones, so
+    // that few vectors still keep all four busy)
+    const uint32_t vg = wave / T::KG, kg = wave % T::KG;
+    const TreeMeta m = find_meta<true>(c, blockIdx.x);
     const uint32_t group = c.heads / c.kv_heads;
     const uint32_t nvec = m.rows * group;
     const uint32_t slices = (nvec + 32 * VG - 1) / (32 * VG);
@@ -532,6 +569,7 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
         page_ids(k + 1);
     };
     page_ids(0);
+#pragma unroll 1
     for (uint32_t k = 0; k < kAhead; ++k) {
         if (k < steps) issue(k);
     }
@@ -613,10 +651,13 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
         if (__builtin_amdgcn_ballot_w64(move) != 0) {
             const float next = move ? ref + mx : m_run;
             const float scale = move ? __builtin_amdgcn_exp2f(m_run - next) : 1.0f;
+            const bool summed = move && m_run > -INFINITY;  // (else there is nothing yet to rescale)
             m_run = next;
             ref = next == -INFINITY ? 0.0f : next;
             l_run *= scale;
-            if constexpr (kAlone) {
+            if (__builtin_amdgcn_ballot_w64(summed) == 0) {
+                // o is 0
+            } else if constexpr (kAlone) {
                 // a wave with the whole register file keeps o in accumulation registers;
                 // multiplied there, or the compiler moves all of it back and forth in
                 // every step.  (The wait: the last products' results, 18 cycles.)
@@ -654,36 +695,36 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
                 v[j] = *(const VRow<NT> *)(vt + (16 * st + (j & 3) + 8 * (j >> 2)) * (D * 2));
             }
             if constexpr (kNext) scores(k, NS / 4 + st * 3 * NS / 8, NS / 4 + (st + 1) * 3 * NS / 8, acc);
-            u32x4 hi, lo;
+            u32x4 w[T::PP];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float a = __builtin_amdgcn_exp2f(d[8 * st + 2 * j]);
-                const float b = __builtin_amdgcn_exp2f(d[8 * st + 2 * j + 1]);
-                hi[j] = pack_bf16x2(a, b);
-                if constexpr (kF32) {
-                    lo[j] = pack_bf16x2(a - bf16lo(hi[j]), b - bf16hi(hi[j]));
-                    sum[j] += a + b;
-                } else {
-                    // the sum is over the probabilities that the product uses
-                    sum[j] += bf16lo(hi[j]) + bf16hi(hi[j]);
+                float a = __builtin_amdgcn_exp2f(d[8 * st + 2 * j]);
+                float b = __builtin_amdgcn_exp2f(d[8 * st + 2 * j + 1]);
+                if constexpr (kF32) sum[j] += a + b;
+#pragma unroll
+                for (int p = 0; p < T::PP; ++p) {
+                    w[p][j] = pack_bf16x2(a, b);
+                    a -= bf16lo(w[p][j]);
+                    b -= bf16hi(w[p][j]);
                 }
+                // (the sum is over the probabilities that the product uses)
+                if constexpr (!kF32) sum[j] += bf16lo(w[0][j]) + bf16hi(w[0][j]);
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const bf16x8 a = v_operand<NT>(v, t);
-                o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, hi), o[t], 0, 0, 0);
-                if constexpr (kF32) {
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, lo), o[t], 0, 0, 0);
+#pragma unroll
+                for (int p = 0; p < T::PP; ++p) {
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, w[p]), o[t], 0, 0, 0);
                 }
             }
         }
         l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         if constexpr (kNext) held = kChains == 2 ? acc[0] + acc[kChains - 1] : acc[0];
     };
-    // steps + 1 barriers for every wave; stage k's scores run in step k, its softmax and
-    // P V in step k + 1
+    // stage k's scores run in step k, its softmax and P V in step k + 1
     if (!live) {
-        for (uint32_t k = 0; k <= steps; ++k) enter(k);
+        for (uint32_t k = 0; k < steps; ++k) enter(k);
     } else {
         enter(0);
         {
@@ -695,52 +736,25 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
             enter(k);
             advance(k, std::true_type{});
         }
-        enter(steps);
         // (the last stage may end before the wave's keys)
         if (key_begin + (steps - 1) * T::kKeys + 32 * kg < key_end) advance(steps, std::false_type{});
     }
-    float l = half_sum(l_run);
-    // join the waves over the keys, through the stages' LDS
-    if constexpr (T::KG > 1) {
-        __syncthreads();
-        float *x = (float *)lds;
-        constexpr uint32_t kWaveFloats = (NT * 16 + 2) * 64;
-        if (kg > 0) {
-            float *w = x + ((kg - 1) * VG + vg) * kWaveFloats + lane;
-            w[0] = m_run;
-            w[64] = l;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) w[(2 + 16 * t + i) * 64] = o[t][i];
-        }
-        __syncthreads();
-        if (kg > 0) return;
-#pragma unroll 1
-        for (int g = 1; g < T::KG; ++g) {
-            const float *w = x + ((g - 1) * VG + vg) * kWaveFloats + lane;
-            const float m2 = w[0], l2 = w[64];
-            const float mx = fmaxf(m_run, m2);
-            const float ref = mx == -INFINITY ? 0.0f : mx;
-            const float s1 = __builtin_amdgcn_exp2f(m_run - ref), s2 = __builtin_amdgcn_exp2f(m2 - ref);
-            m_run = mx;
-            l = l * s1 + l2 * s2;
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[t][i] = o[t][i] * s1 + w[(2 + 16 * t + i) * 64] * s2;
-        }
-    }
-    if (!live || tile * 32 + col >= nvec) return;
-    const uint32_t head = kvh * group + vec % group;
-    const size_t out_row = (size_t)(m.row0 + row) * c.heads + head;
-    if (c.records != nullptr) {
-        float *rec = c.records + ((size_t)m.record0 + ((size_t)row * c.heads + head) * m.parts + part) *
-                                     tree_record_floats(D);
-        if (h == 0) *(float2 *)rec = make_float2(m_run, l);
+    // The waves over the keys are joined through LDS, a record per query vector and wave
+    // in the place of the stages: {m, l, -, -, o}.  Then each of them finishes its share
+    // of the vectors, a row at a time and as loops: a launch begins with no code in the
+    // instruction cache, and code that runs once costs its fetch.
+    constexpr uint32_t kRecord = tree_record_floats(D);
+    float *joined = (float *)lds + (size_t)vg * 32 * kRecord;  // of wave (vg, kg 0)
+    constexpr uint32_t kNextWave = VG * 32 * kRecord;
+    static_assert(sizeof(float) * kNextWave * T::KG <= T::kLds, "records fit the stages");
+    const float l = half_sum(l_run);
+    __syncthreads();
+    if (live) {
+        float *w = joined + kg * kNextWave + col * kRecord;
+        if (h == 0) *(float2 *)w = make_float2(m_run, l);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            float *dst = rec + 4 + NT * (8 * (i >> 2) + 4 * h + (i & 3));
+            float *dst = w + 4 + NT * (8 * (i >> 2) + 4 * h + (i & 3));
             if constexpr (NT == 2) {
                 *(float2 *)dst = make_float2(o[0][i], o[1][i]);
             } else {
@@ -748,26 +762,53 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
                 for (int t = 0; t < NT; t += 4) *(float4 *)(dst + t) = make_float4(o[t][i], o[t + 1][i], o[t + 2][i], o[t + 3][i]);
             }
         }
-        return;
     }
+    __syncthreads();
+    if (!live) return;
     const bool gated = (c.flags & SAFETYRAISE_MI355X_GATED) != 0;
     const bool bf16_in = (c.flags & SAFETYRAISE_MI355X_INPUT_BF16) != 0;
     const bool out16 = (c.flags & SAFETYRAISE_MI355X_OUTPUT_BF16) != 0;
-    const float inv = 1.0f / l;
+    constexpr uint32_t kRows = 256 / D;  // rows at a time: a lane has 4 dims of one
+    constexpr uint32_t kShare = 32 / T::KG;
+    const uint32_t d = 4 * (lane % (D / 4));
+    const uint32_t left = min(32u, nvec - tile * 32);
+#pragma unroll 1
+    for (uint32_t i = kg * kShare + lane / (D / 4); i < min(left, (kg + 1) * kShare); i += kRows) {
+        const float *w = joined + i * kRecord;
+        float2 ml = *(const float2 *)w;
+        f32x4 y = *(const f32x4 *)(w + 4 + d);
+        if constexpr (T::KG > 1) {
+            float mx = ml.x;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const uint32_t d = NT * (8 * (i >> 2) + 4 * h + (i & 3));
-        float y[NT];
+            for (int g = 1; g < T::KG; ++g) mx = fmaxf(mx, w[g * kNextWave]);
+            const float ref = mx == -INFINITY ? 0.0f : mx;
+            const float first = __builtin_amdgcn_exp2f(ml.x - ref);
+            ml = make_float2(mx, ml.y * first);
+            y *= first;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            y[t] = o[t][i] * inv;
-            if (gated) y[t] *= ref_sigmoid(load_act(c.q, out_row * 2 * D + D + d + t, bf16_in));
+            for (int g = 1; g < T::KG; ++g) {
+                const float2 next = *(const float2 *)(w + g * kNextWave);
+                const float weight = __builtin_amdgcn_exp2f(next.x - ref);
+                ml.y = fmaf(next.y, weight, ml.y);
+                y += *(const f32x4 *)(w + g * kNextWave + 4 + d) * weight;
+            }
         }
-#pragma unroll
-        for (int t = 0; t < NT; t += 2) {
-            if (out16) *(uint32_t *)((uint16_t *)c.out + out_row * D + d + t) = pack_bf16x2(y[t], y[t + 1]);
-            else *(float2 *)((float *)c.out + out_row * D + d + t) = make_float2(y[t], y[t + 1]);
+        const uint32_t v = tile * 32 + i, r = v / group, head = kvh * group + v % group;
+        if (c.records != nullptr) {
+            float *rec = c.records + ((size_t)m.record0 + ((size_t)r * c.heads + head) * m.parts + part) * kRecord;
+            if (d == 0) *(float2 *)rec = ml;
+            *(f32x4 *)(rec + 4 + d) = y;
+            continue;
         }
+        const size_t out_row = (size_t)(m.row0 + r) * c.heads + head;
+        y *= 1.0f / ml.y;
+        if (gated) {
+            const size_t gate = out_row * 2 * D + D + d;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] *= ref_sigmoid(load_act(c.q, gate + j, bf16_in));
+        }
+        if (out16) *(uint2 *)((uint16_t *)c.out + out_row * D + d) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+        else *(f32x4 *)((float *)c.out + out_row * D + d) = y;
     }
 }
 
@@ -780,8 +821,7 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeCommon c, u
     const uint32_t w = blockIdx.x * 4 + (uint32_t)wave_index();
     if (w >= rows * c.heads) return;
     const uint32_t r = w / c.heads, head = w % c.heads;
-    const uint32_t s = find_row(c, r);
-    const TreeMeta m = c.meta[s];
+    const TreeMeta m = find_meta<false>(c, r);
     const uint32_t sr = r - (m.row0 - c.meta[0].row0);
     const float *rec = c.records + ((size_t)m.record0 + ((size_t)sr * c.heads + head) * m.parts) * tree_record_floats(D);
     float mx = -INFINITY;
