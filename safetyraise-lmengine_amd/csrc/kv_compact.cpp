@@ -164,7 +164,8 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
     std::vector<KnownPlan> known;
     std::vector<uint32_t> plan_of(n);
     size_t ranges = 0, links = 0, words = 0;
-    uint32_t chains = 0, kv_heads = 1;
+    uint32_t chains = 0, kv_heads = 1, in_flight = UINT32_MAX;
+    uint64_t longest = 1;
     for (uint32_t i = 0; i < n; ++i) {
         const auto &e = entries[i];
         Pool *pool = e.kv;
@@ -197,7 +198,10 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
         chains += (uint32_t)(p.serial ? std::min<size_t>(p.ranges.size(), 1) : p.ranges.size());
         links += p.take.empty() ? 0 : 1;
         words += p.take.size();
-        if (!p.ranges.empty()) kv_heads = std::max(kv_heads, pool->kv_heads);
+        if (p.ranges.empty()) continue;
+        kv_heads = std::max(kv_heads, pool->kv_heads);
+        in_flight = std::min(in_flight, move_rows(pool->head_dim));
+        for (const auto &r : p.ranges) longest = std::max(longest, r.end - r.begin);
     }
     const size_t fixed = (n * sizeof(MoveEntry) + ranges * sizeof(MoveRange) + links * sizeof(MoveLink)) / 4;
     words += fixed;
@@ -300,7 +304,9 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
     call.chains = chains;
     call.ranges = (uint32_t)ranges;
     call.late_links = (uint32_t)late.size();
-    call.kv_heads = kv_heads;
+    // short ranges: a workgroup takes as many heads as it has in flight at once
+    while ((2u << call.log2_heads) <= kv_heads && (longest << (call.log2_heads + 1)) <= in_flight) ++call.log2_heads;
+    call.head_groups = (kv_heads + (1u << call.log2_heads) - 1) >> call.log2_heads;
     call.host_words = w.at;
     call.words = (uint32_t)(list - w.at);
     if (call.chains + call.links + call.late_links > 0) {

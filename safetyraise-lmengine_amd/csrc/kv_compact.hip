@@ -16,57 +16,62 @@ typedef uint32_t Unit16 __attribute__((ext_vector_type(4)));  // 8 values
 
 struct MoveArgs {
     const uint32_t *words;  // nullptr: inline_words
-    uint32_t entries, ranges, chains, links;
+    uint32_t entries, ranges, chains, links, log2_heads;
     alignas(16) uint32_t inline_words[kMoveInlineWords];
 };
 static_assert(sizeof(MoveArgs) <= 4096, "kernel arguments stay within 4 KiB");
 
-// A workgroup moves the tokens of one range of one head's K or V, in the order
-// of the tokens: a chunk is read whole before any of it is written.  A row is `per`
-// units; a thread has one of them in every pass of 256 / per rows (rows of more than
-// 256 units: 256 / per is 0, and a thread takes every 256th unit of one row).
-template <typename Unit, uint32_t kPasses>
+// A workgroup moves the tokens of one range, K or V of 2^lh heads, in the order of the
+// tokens: a chunk is read whole before any of it is written.  A row (one token of one
+// head) is `per` units; a thread has one of them in every pass of 256 / per rows (rows
+// of more than 256 units: a thread takes every 256th unit of one row).
+template <typename Unit>
 __device__ __forceinline__ void move_range(uint16_t *pages, const MoveEntry &e, const MoveRange &r,
                                            const int32_t *from, const int32_t *to,
-                                           const uint32_t *tokens, uint32_t kvh) {
+                                           const uint32_t *tokens, uint32_t head0, uint32_t lh) {
     const uint32_t per = (uint32_t)(e.head_dim * 2 / sizeof(Unit));  // at most 512 units
     const uint32_t lpt = e.log2_page, mask = (1u << lpt) - 1;
-    Unit *base = global_from_bits<Unit>((uint64_t)(pages + (((size_t)kvh * e.num_pages) << lpt) * e.head_dim));
+    Unit *base = global_from_bits<Unit>((uint64_t)pages);
+    const size_t head_rows = (size_t)e.num_pages << lpt;
     const uint32_t rows = per <= 256 ? 256 / per : 1;  // of a pass
     const uint32_t my_row = per <= 256 ? threadIdx.x / per : 0;
     const uint32_t my_unit = per <= 256 ? threadIdx.x % per : threadIdx.x;
-    for (uint32_t t0 = r.begin; t0 < r.end; t0 += rows * kPasses) {
+    const uint32_t chunk = max(1u, (rows * kMovePasses) >> lh);  // tokens
+    for (uint32_t t0 = r.begin; t0 < r.end; t0 += chunk) {
         for (uint32_t u0 = 0; u0 < per; u0 += 256) {  // (once, but for rows of more than 256 units)
             const uint32_t u = min(u0 + my_unit, per - 1);
-            Unit x[kPasses];
-            Unit *dst[kPasses];
-            bool ok[kPasses];
-            uint32_t s[kPasses];
+            Unit x[kMovePasses];
+            Unit *dst[kMovePasses];
+            bool ok[kMovePasses];
+            uint32_t s[kMovePasses];
+            size_t head[kMovePasses];
 #pragma unroll
-            for (uint32_t i = 0; i < kPasses; ++i) {
-                const uint32_t t = t0 + rows * i + my_row;
-                ok[i] = my_row < rows && u0 + my_unit < per && t < r.end;
+            for (uint32_t i = 0; i < kMovePasses; ++i) {
+                const uint32_t at = rows * i + my_row, t = t0 + (at >> lh);
+                const uint32_t hh = head0 + (at & ((1u << lh) - 1));
+                ok[i] = my_row < rows && u0 + my_unit < per && (at >> lh) < chunk && t < r.end && hh < e.kv_heads;
                 const uint32_t tc = ok[i] ? t : r.begin;
+                head[i] = (ok[i] ? hh : head0) * head_rows;
                 s[i] = tc < e.start ? tc : e.start + tokens[tc - e.start];
-                dst[i] = base + (((size_t)to[(tc >> lpt) - e.first_page] << lpt) + (tc & mask)) * per + u;
+                dst[i] = base + (head[i] + ((size_t)to[(tc >> lpt) - e.first_page] << lpt) + (tc & mask)) * per + u;
             }
 #pragma unroll
-            for (uint32_t i = 0; i < kPasses; ++i) {
-                x[i] = base[(((size_t)from[s[i] >> lpt] << lpt) + (s[i] & mask)) * per + u];
+            for (uint32_t i = 0; i < kMovePasses; ++i) {
+                x[i] = base[(head[i] + ((size_t)from[s[i] >> lpt] << lpt) + (s[i] & mask)) * per + u];
             }
             // every wave's reads are done before any wave writes
             __builtin_amdgcn_s_waitcnt(0x0F70);
             __syncthreads();
 #pragma unroll
-            for (uint32_t i = 0; i < kPasses; ++i) {
+            for (uint32_t i = 0; i < kMovePasses; ++i) {
                 if (ok[i]) *dst[i] = x[i];
             }
         }
     }
 }
 
-// grid (range that begins a chain, 2 x KV heads); then links: blocks past the ranges write page-table
-// rows of targets that no range reads
+// grid (range that begins a chain, 2 x groups of heads); then links: blocks past the
+// ranges write page-table rows of targets that no range reads
 __global__ void __launch_bounds__(256) kv_move_kernel(const MoveArgs a) {
     const uint32_t *w = a.words != nullptr ? a.words : a.inline_words;
     const MoveEntry *entries = (const MoveEntry *)w;
@@ -80,14 +85,14 @@ __global__ void __launch_bounds__(256) kv_move_kernel(const MoveArgs a) {
     MoveRange r = ranges[blockIdx.x];
     const MoveEntry e = entries[r.entry];
     const int32_t *from = global_from_bits<const int32_t>((uint64_t)e.from);
-    const uint32_t kvh = blockIdx.y >> 1;
-    if (kvh >= e.kv_heads) return;
+    const uint32_t head0 = (blockIdx.y >> 1) << a.log2_heads;
+    if (head0 >= e.kv_heads) return;
     uint16_t *pages = (blockIdx.y & 1) ? e.v_pages : e.k_pages;
     const int32_t *to = (const int32_t *)(w + e.pages);
     const uint32_t *tokens = w + e.tokens;
     for (;;) {
-        if (e.head_dim % 8 == 0) move_range<Unit16, 4>(pages, e, r, from, to, tokens, kvh);
-        else move_range<uint16_t, 4>(pages, e, r, from, to, tokens, kvh);
+        if (e.head_dim % 8 == 0) move_range<Unit16>(pages, e, r, from, to, tokens, head0, a.log2_heads);
+        else move_range<uint16_t>(pages, e, r, from, to, tokens, head0, a.log2_heads);
         if (r.next == 0) break;
         r = ranges[r.next];
     }
@@ -184,12 +189,13 @@ hipError_t launch_kv_moves(hipStream_t stream, const MoveCall &c) {
     a.ranges = c.ranges;
     a.chains = c.chains;
     a.links = c.links;
+    a.log2_heads = c.log2_heads;
     if (a.words == nullptr) {
         if (c.words > kMoveInlineWords) return hipErrorInvalidValue;
         for (uint32_t i = 0; i < c.words; ++i) a.inline_words[i] = c.host_words[i];
     }
     if (c.chains + c.links > 0) {
-        SR_LAUNCH("kv_move_kernel", kv_move_kernel, dim3(c.chains + c.links, 2 * c.kv_heads), dim3(256),
+        SR_LAUNCH("kv_move_kernel", kv_move_kernel, dim3(c.chains + c.links, 2 * c.head_groups), dim3(256),
                   0, stream, a);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;

@@ -50,6 +50,13 @@ static_assert(sizeof(MoveEntry) % 8 == 0 && sizeof(MoveRange) % 8 == 0 && sizeof
 constexpr uint32_t kMoveInlineWords = 1008;  // what fits the kernel arguments
 constexpr uint32_t kGatherInlineWords = 992;
 
+// Rows (one token of one head) that a workgroup of the move kernel has in flight.
+constexpr uint32_t kMovePasses = 4;
+constexpr uint32_t move_rows(uint32_t head_dim) {
+    const uint32_t units = head_dim % 8 == 0 ? head_dim / 8 : head_dim;
+    return kMovePasses * (units <= 256 ? 256 / units : 1);
+}
+
 struct MoveCall {
     const uint32_t *host_words;
     const uint32_t *device_words;  // nullptr: the words travel in the arguments
@@ -57,7 +64,7 @@ struct MoveCall {
     uint32_t entries, ranges, chains;
     uint32_t links;       // rows that no range of the call reads
     uint32_t late_links;  // rows written after the ranges
-    uint32_t kv_heads;
+    uint32_t log2_heads, head_groups;  // a workgroup moves 2^log2_heads heads of a range
 };
 struct GatherCall {
     const uint32_t *host_words;
