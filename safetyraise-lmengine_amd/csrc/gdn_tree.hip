@@ -231,12 +231,20 @@ constexpr uint32_t kHist = 7;        // history rows in front of the tree's
 template <int RT>
 struct HeadShape {
     static constexpr uint32_t kRows = 16 * RT;
-    static constexpr uint32_t kPart = (kHist + kRows) * kPitch;  // floats of q, k or v
+    static constexpr uint32_t kPart = (kHist + kRows) * kPitch;  // floats of raw q, k or v
     static constexpr uint32_t kPair = kRows + 4;                 // pitch of A and P
-    static constexpr size_t kLds = (3 * kPart + 2 * kRows * kPair) * sizeof(float);
+    // raw q, k, v, and the finished v; the finished q is where v was, the finished k
+    // where q was, A and P where k was
+    static constexpr size_t kLds = (3 * kPart + kRows * kPitch) * sizeof(float);
+    static_assert(2 * kRows * kPair <= kPart, "A and P fit the raw k");
 };
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+// (the records' rows are aligned to 4 bytes only)
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -291,8 +299,8 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
     __shared__ float beta_s[kRowsMax], decay_s[kRowsMax];
     // a row's conv taps, newest first: byte offsets of their LDS rows
     __shared__ __align__(16) uint16_t tap_s[kRowsMax][8];
-    float *xq = lds, *xk = lds + T::kPart, *xv = lds + 2 * T::kPart;
-    float *As = lds + 3 * T::kPart, *Ps = As + T::kRows * kPair;
+    float *xq = lds + 2 * T::kPart, *xk = lds, *xv = lds + 3 * T::kPart;
+    float *As = lds + T::kPart, *Ps = As + T::kRows * kPair;
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = (uint32_t)wave_index();
     const uint32_t h = blockIdx.x;
@@ -305,64 +313,91 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
     const uint32_t l16 = lane & 15, g4 = lane >> 4;
     float *rec = p.records + (size_t)m.slot * p.keep_rows * p.rec_stride;
 
-    // 1.
-    const uint32_t part = wave >> 1, c = tid & 127;  // q, k, v; waves 6 and 7 have no channel
-    const uint32_t ch = part == 0 ? kh * kW + c
-                      : part == 1 ? (p.key_heads + kh) * kW + c
-                                  : 2 * p.key_heads * kW + h * kW + c;
-    float *X = lds + part * T::kPart + c;
-    // the wave's state rows: row 16 w + l16, dims 32 s + 8 g4 .. + 7, requested behind the
-    // inputs, which are waited for first
+    // 1. 4 channels of a row per lane: rows 2 n, 2 n + 1 of q, k or v per load
+    const uint32_t l32 = lane & 31, half = lane >> 5;
+    const uint32_t head_ch[3] = {kh * kW, (p.key_heads + kh) * kW, 2 * p.key_heads * kW + h * kW};
+    const uint32_t r = min(lane, R - 1);
+    const size_t ab_at = (size_t)(m.row0 + r) * p.value_heads + h;
+    uint32_t a_raw = 0, b_raw = 0, up_raw = 0;
+    float a_log = 0.0f, dt_bias = 0.0f;
+    if (wave == 0) {
+        a_raw = ((const uint32_t *)p.a)[bf16 ? ab_at >> 1 : ab_at];
+        b_raw = ((const uint32_t *)p.b)[bf16 ? ab_at >> 1 : ab_at];
+        // (a lane's loads: scalar ones would be waited for here)
+        uint32_t at = h;
+        asm volatile("" : "+v"(at));
+        a_log = p.a_log[at];
+        dt_bias = p.dt_bias[at];
+        up_raw = p.parent[m.row0 - p.meta[0].row0 + r];
+    }
+    u32x4 raw[3 * RT];
+    u32x2 raw16[3 * RT];
+    auto raw_at = [&](int n) __attribute__((always_inline)) {
+        const uint32_t row = min(2 * (wave + 8 * (n % RT)) + half, R - 1);
+        return (size_t)(m.row0 + row) * p.channels + head_ch[n / RT] + 4 * l32;
+    };
+    if (bf16) {
+#pragma unroll
+        for (int n = 0; n < 3 * RT; ++n) raw16[n] = *(const u32x2 *)((const uint16_t *)p.qkv + raw_at(n));
+    } else {
+#pragma unroll
+        for (int n = 0; n < 3 * RT; ++n) raw[n] = *(const u32x4 *)((const float *)p.qkv + raw_at(n));
+    }
+    // the channels' history, one per thread
+    const uint32_t hc = tid & 127, hpart = min(tid >> 7, 2u);
+    float old[kHist];
+    {
+        const uint32_t ch = hc + (hpart < 2 ? (hpart * p.key_heads + kh) * kW : 2 * p.key_heads * kW + h * kW);
+        const float *hist = p.history + (((size_t)m.parity * p.max_slots + m.slot) * p.channels + ch) * K1;
+#pragma unroll
+        for (uint32_t j = 0; j < kHist; ++j) old[j] = j < K1 ? hist[j] : 0.0f;
+    }
+    // conv weights of channels 2 lane, 2 lane + 1, oldest tap first: of 4 taps, or any
+    // (in registers of their own, or the loads of one kind would wait for the other's)
+    f32x4 w4[3][2];
+    float w[3][8][2];
+    if (K == 4) {
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                w4[part][e] = *(const f32x4u *)(p.conv_w + (size_t)(head_ch[part] + 2 * lane + e) * 4);
+            }
+    }
+    if (K != 4) {
+#pragma unroll
+        for (int part = 0; part < 3; ++part)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float *src = p.conv_w + (size_t)(head_ch[part] + 2 * lane + e) * K;
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) w[part][j][e] = j < K ? src[j] : 0.0f;
+            }
+    }
+    // the wave's state rows: row 16 w + l16, dims 32 s + 8 g4 .. + 7
     f32x4 S[8];
-    auto load_state = [&]() __attribute__((always_inline)) {
+    {
         const float *src = p.state + (((size_t)m.state_in * p.value_heads + h) * kW + 16 * wave + l16) * kW + 8 * g4;
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
             S[s] = __builtin_nontemporal_load((const f32x4 *)(src + 32 * (s >> 1) + 4 * (s & 1)));
         }
-    };
-    float w[8];
-    if (part < 3) {
-        const float *hist = p.history + (((size_t)m.parity * p.max_slots + m.slot) * p.channels + ch) * K1;
-        float x[T::kRows], old[kHist];
-#pragma unroll
-        for (uint32_t i = 0; i < T::kRows; ++i) {
-            x[i] = load_act_nb(p.qkv, (size_t)(m.row0 + min(i, R - 1)) * p.channels + ch, bf16);
-        }
-        // (the history holds at least one value, also for K = 1)
-#pragma unroll
-        for (uint32_t j = 0; j < kHist; ++j) old[j] = hist[j < K1 ? j : 0];
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) {
-            const float x = p.conv_w[(size_t)ch * K + (j < K ? K1 - j : 0)];  // newest first
-            w[j] = j < K ? x : 0.0f;
-        }
-        load_state();
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (uint32_t j = 0; j < kHist; ++j) {
-            if (j < K1) X[(kHist - K1 + j) * kPitch] = old[j];
-        }
-        const bool owns = part == 2 || first_of_key;
-#pragma unroll
-        for (uint32_t i = 0; i < T::kRows; ++i) {
-            X[(kHist + i) * kPitch] = i < R ? x[i] : 0.0f;
-            if (owns && i < R) rec[(size_t)i * p.rec_stride + rec_raw(p) + ch] = x[i];
-        }
-    } else if (wave == 6) {
-        const uint32_t r = min(lane, R - 1);
-        const float av = load_act(p.a, (size_t)(m.row0 + r) * p.value_heads + h, bf16);
-        const float bv = load_act(p.b, (size_t)(m.row0 + r) * p.value_heads + h, bf16);
-        load_state();
-        __builtin_amdgcn_sched_barrier(0);
-        const int up = (int)p.parent[m.row0 - p.meta[0].row0 + r] - 1;
-        const float log_a = -expf(p.a_log[h]) * softplus_ref(av + p.dt_bias[h]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (wave == 0) {
+        // (used from here on: earlier, the compiler would wait for them before the other loads)
+        asm volatile("" : "+v"(up_raw), "+v"(a_log), "+v"(dt_bias));
+        const bool high = bf16 && (ab_at & 1);
+        const float av = !bf16 ? __uint_as_float(a_raw) : high ? bf16hi(a_raw) : bf16lo(a_raw);
+        const float bv = !bf16 ? __uint_as_float(b_raw) : high ? bf16hi(b_raw) : bf16lo(b_raw);
+        const int up = (int)up_raw - 1;
+        const float log_a = -expf(a_log) * softplus_ref(av + dt_bias);
         // the path's set and sum up to, not with, `next`: doubling
         int next = up;
         uint32_t lo = r < 32 ? 1u << r : 0u, hi = r < 32 ? 0u : 1u << (r - 32);
         double sum = (double)log_a;
-#pragma unroll
-        for (int step = 0; step < 6; ++step) {
+#pragma unroll 1
+        for (int step = 0; step < 6 && __builtin_amdgcn_ballot_w64(next >= 0) != 0; ++step) {
             const int at = next < 0 ? (int)lane : next;
             const uint32_t l2 = __shfl(lo, at), h2 = __shfl(hi, at);
             const double s2 = __shfl(sum, at);
@@ -375,13 +410,14 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
             }
         }
         int at = (int)r, back = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) {
+#pragma unroll 1
+        for (uint32_t j = 0; j < (K == 4 ? 4u : 8u); ++j) {
             // past the kernel's taps: any finite row, its weight is 0
             if (j >= K) at = (int)r;
             if (lane >= R) at = (int)lane;
             const int u = __shfl(up, at < 0 ? 0 : at);
-            tap_s[lane][j] = (uint16_t)((at >= 0 ? (int)kHist + at : (int)kHist - 1 - back) * (int)(kPitch * 4));
+            tap_s[lane][j < K ? K1 - j : j] =
+                (uint16_t)((at >= 0 ? (int)kHist + at : (int)kHist - 1 - back) * (int)(kPitch * 4));
             back += at < 0 ? 1 : 0;
             at = at < 0 ? -1 : u;
         }
@@ -397,83 +433,113 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
             anc_s[lane] = 0;
             beta_s[lane] = decay_s[lane] = 0.0f;
         }
-    } else {
-        load_state();
     }
-    // 8. barrier
+#pragma unroll
+    for (int n = 0; n < 3 * RT; ++n) {
+        const uint32_t row = 2 * (wave + 8 * (n % RT)) + half;
+        f32x4 x;
+        if (bf16) x = f32x4{bf16lo(raw16[n].x), bf16hi(raw16[n].x), bf16lo(raw16[n].y), bf16hi(raw16[n].y)};
+        else x = __builtin_bit_cast(f32x4, raw[n]);
+        if (row >= R) x = f32x4{};
+        *(f32x4 *)(lds + (n / RT) * T::kPart + (kHist + row) * kPitch + 4 * l32) = x;
+        if ((n / RT == 2 || first_of_key) && row < R) {
+            *(f32x4u *)(rec + (size_t)row * p.rec_stride + rec_raw(p) + head_ch[n / RT] + 4 * l32) = x;
+        }
+    }
+    if (tid < 3 * kW) {
+#pragma unroll
+        for (uint32_t j = 0; j < kHist; ++j) {
+            if (j < K1) lds[hpart * T::kPart + (kHist - K1 + j) * kPitch + hc] = old[j];
+        }
+    }
     __syncthreads();
-    // 2. oldest tap first, as the reference sums them (math.rs:175-185); rows past the
-    // tree are zeros with themselves as taps
-    if (part < 3) {
-        auto conv = [&](auto taps_of) __attribute__((always_inline)) {
-            constexpr uint32_t KT = decltype(taps_of)::value;  // taps read per row
-            constexpr int kBatch = KT == 4 ? 8 : 4;            // rows whose reads are in flight
-            for (int t0 = 16 * (int)rt - kBatch; t0 >= 0; t0 -= kBatch) {
+    // 2., 3. v, then q, then k, each into memory that no row reads any more: kBatch rows
+    // per wave at a time, two channels per lane.  Oldest tap first, as the reference sums
+    // them (math.rs:175-185); rows past the tree are zeros with themselves as taps
+    float *const keys = rec + rec_key(p) + kh * kW + 2 * lane;
+    const uint32_t rec_stride = p.rec_stride;
+    auto conv = [&](auto taps_of) __attribute__((always_inline)) {
+        constexpr uint32_t KT = decltype(taps_of)::value;  // taps read per row
+        constexpr uint32_t kBatch = 2 * RT < 4 ? 2 * RT : 4;
+#pragma unroll 1
+        for (int turn = 0; turn < 3; ++turn) {
+            const int part = turn == 0 ? 2 : turn - 1;
+            const float *from = lds + part * T::kPart + 2 * lane;
+            float *to = lds + (turn == 0 ? 3u : turn == 1 ? 2u : 0u) * T::kPart;  // xv, xq, xk
+            // (by value: a choice between array elements would put the array in memory)
+            auto of_turn = [turn](float first, float second, float third) {
+                return turn == 0 ? first : turn == 1 ? second : third;
+            };
+            float wt[KT][2];
+#pragma unroll
+            for (uint32_t j = 0; j < KT; ++j)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if constexpr (KT == 4) wt[j][e] = of_turn(w4[2][e][j], w4[0][e][j], w4[1][e][j]);
+                    else wt[j][e] = of_turn(w[2][j][e], w[0][j][e], w[1][j][e]);
+                }
+            for (uint32_t t0 = wave; t0 < 16 * rt; t0 += 8 * kBatch) {
                 uint32_t tap[kBatch][KT / 2];
-                float x[kBatch][KT];
+                float2 x[kBatch][KT];
+                // (past the last tile: the batch's first row again)
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i)
+                for (uint32_t i = 0; i < kBatch; ++i) {
+                    const uint32_t t = t0 + 8 * i < 16 * rt ? t0 + 8 * i : t0;
 #pragma unroll
-                    for (uint32_t j = 0; j < KT / 2; ++j) tap[i][j] = ((const uint32_t *)tap_s[t0 + i])[j];
-                __builtin_amdgcn_sched_barrier(0);
+                    for (uint32_t j = 0; j < KT / 2; ++j) tap[i][j] = ((const uint32_t *)tap_s[t])[j];
+                }
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i)
+                for (uint32_t i = 0; i < kBatch; ++i)
 #pragma unroll
                     for (uint32_t j = 0; j < KT / 2; ++j) {
                         const uint32_t two = (uint32_t)__builtin_amdgcn_readfirstlane((int)tap[i][j]);
-                        x[i][2 * j] = *(const float *)((const char *)X + (two & 0xffffu));
-                        x[i][2 * j + 1] = *(const float *)((const char *)X + (two >> 16));
+                        x[i][2 * j] = *(const float2 *)((const char *)from + (two & 0xffffu));
+                        x[i][2 * j + 1] = *(const float2 *)((const char *)from + (two >> 16));
                     }
                 __builtin_amdgcn_sched_barrier(0);
+                float2 y[kBatch];
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i) {
-                    float acc = 0.0f;
+                for (uint32_t i = 0; i < kBatch; ++i) {
+                    float a = 0.0f, b = 0.0f;
 #pragma unroll
                     for (uint32_t j = 0; j < KT; ++j) {
-                        // (weights past the kernel's are 0)
-                        acc = fmaf(x[i][KT - 1 - j], w[KT - 1 - j], acc);
+                        a = fmaf(x[i][j].x, wt[j][0], a);
+                        b = fmaf(x[i][j].y, wt[j][1], b);
                     }
-                    x[i][0] = acc;
+                    y[i] = make_float2(silu_fast(a), silu_fast(b));
                 }
+                if (turn == 0) {
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i) X[(kHist + t0 + i) * kPitch] = silu_fast(x[i][0]);
-            }
-        };
-        if (K <= 4) conv(std::integral_constant<uint32_t, 4>{});
-        else conv(std::integral_constant<uint32_t, 8>{});
-    }
-    __syncthreads();
-    // 3. four vectors of a wave at a time; past the last, the last again
-    for (uint32_t t0 = wave; t0 < 2 * R; t0 += 32) {
-        float2 y[4];
-        float inv[4];
-        float *row[4];
+                    for (uint32_t i = 0; i < kBatch; ++i) {
+                        if (t0 + 8 * i < 16 * rt) *(float2 *)(to + (t0 + 8 * i) * kPitch + 2 * lane) = y[i];
+                    }
+                    continue;
+                }
+                float inv[kBatch];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t t = min(t0 + 8 * i, (t0 & 1) + 2 * R - 2);
-            row[i] = ((t & 1) ? xk : xq) + (kHist + (t >> 1)) * kPitch;
-            y[i] = *(const float2 *)(row[i] + 2 * lane);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+                for (uint32_t i = 0; i < kBatch; ++i) inv[i] = fmaf(y[i].y, y[i].y, y[i].x * y[i].x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) inv[i] = fmaf(y[i].y, y[i].y, y[i].x * y[i].x);
+                for (uint32_t i = 0; i < kBatch; ++i) inv[i] = __builtin_amdgcn_rsqf(wave_sum(inv[i]) + 1e-6f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) inv[i] = __builtin_amdgcn_rsqf(wave_sum(inv[i]) + 1e-6f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float a = y[i].x * inv[i], b = y[i].y * inv[i];
-            constexpr float kScale = (float)(1 << kSplitExp);
-            const f16x2 hi = {(_Float16)(a * kScale), (_Float16)(b * kScale)};
-            const f16x2 lo = {(_Float16)(a * kScale - (float)hi.x), (_Float16)(b * kScale - (float)hi.y)};
-            if (t0 + 8 * i < 2 * R) {
-                ((f16x2 *)row[i])[lane] = hi;
-                ((f16x2 *)row[i])[64 + lane] = lo;
-                if ((t0 & 1) && first_of_key) {
-                    *(float2 *)(rec + (size_t)((t0 + 8 * i) >> 1) * p.rec_stride + rec_key(p) + kh * kW + 2 * lane) = make_float2(a, b);
+                for (uint32_t i = 0; i < kBatch; ++i) {
+                    const uint32_t t = t0 + 8 * i;
+                    if (t >= 16 * rt) break;
+                    const float a = y[i].x * inv[i], b = y[i].y * inv[i];
+                    constexpr float kScale = (float)(1 << kSplitExp);
+                    const f16x2 hi = {(_Float16)(a * kScale), (_Float16)(b * kScale)};
+                    const f16x2 lo = {(_Float16)(a * kScale - (float)hi.x), (_Float16)(b * kScale - (float)hi.y)};
+                    ((f16x2 *)(to + t * kPitch))[lane] = hi;
+                    ((f16x2 *)(to + t * kPitch))[64 + lane] = lo;
+                    if (turn == 2 && first_of_key && t < R) {
+                        *(f32x2u *)(keys + (size_t)t * rec_stride) = f32x2u{a, b};
+                    }
                 }
             }
+            __syncthreads();
         }
-    }
+    };
+    if (K == 4) conv(std::integral_constant<uint32_t, 4>{});
+    else conv(std::integral_constant<uint32_t, 8>{});
     // the state rows' parts
     Split Sp[4];
     int back;  // exponent that undoes the scales
@@ -498,17 +564,28 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
                 Sp[s >> 1].lo[4 * (s & 1) + i] = (_Float16)(x - (float)hi);
             }
     }
-    __syncthreads();
-    // 4.
+    // 4. a wave reads every block of k and q for its state rows; on the way block `mine`
+    // of k (even waves) or q meets the blocks of k up to it
     f32x4 kS[RT], qS[RT];
+    const uint32_t mine = wave >> 1;
+    const bool is_q = (wave & 1) != 0;
+    Split own[4];
+    {
+        const float *ar = (is_q ? xq : xk) + (16 * min(mine, rt - 1) + l16) * kPitch;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) own[s] = split_row(ar, 32 * s + 8 * g4);
+    }
 #pragma unroll
     for (int b = 0; b < RT; ++b) {
         kS[b] = qS[b] = f32x4{};
         if ((uint32_t)b >= rt) continue;
-        const float *kr = xk + (kHist + 16 * b + l16) * kPitch, *qr = xq + (kHist + 16 * b + l16) * kPitch;
+        const float *kr = xk + (16 * b + l16) * kPitch, *qr = xq + (16 * b + l16) * kPitch;
+        f32x4 acc[2] = {f32x4{}, f32x4{}};
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-            kS[b] = mma_split(split_row(kr, 32 * s + 8 * g4), Sp[s], kS[b]);
+            const Split kf = split_row(kr, 32 * s + 8 * g4);
+            kS[b] = mma_split(kf, Sp[s], kS[b]);
+            acc[s & 1] = mma_split(own[s], kf, acc[s & 1]);
             qS[b] = mma_split(split_row(qr, 32 * s + 8 * g4), Sp[s], qS[b]);
         }
 #pragma unroll
@@ -516,26 +593,12 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
             kS[b][e] = __builtin_amdgcn_ldexpf(kS[b][e], back);
             qS[b][e] = __builtin_amdgcn_ldexpf(qS[b][e], back);
         }
-    }
-    {
-        // blocks (bt, bj), bj <= bt, of K K^T, then of Q K^T
-        const uint32_t blocks = rt * (rt + 1);
-        for (uint32_t i = wave; i < blocks; i += 8) {
-            const bool is_q = i >= blocks / 2;
-            uint32_t bj = is_q ? i - blocks / 2 : i, bt = 0;
-            while (bj > bt) bj -= ++bt;
-            const float *ar = (is_q ? xq : xk) + (kHist + 16 * bt + l16) * kPitch;
-            const float *br = xk + (kHist + 16 * bj + l16) * kPitch;
-            f32x4 acc[2] = {f32x4{}, f32x4{}};
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                acc[s & 1] = mma_split(split_row(ar, 32 * s + 8 * g4), split_row(br, 32 * s + 8 * g4), acc[s & 1]);
-            }
-            const uint32_t j = 16 * bj + l16;
+        if (mine < rt && (uint32_t)b <= mine) {
+            const uint32_t j = 16 * b + l16;
             const double gj = g_s[j];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t t = 16 * bt + 4 * g4 + e;
+                const uint32_t t = 16 * mine + 4 * g4 + e;
                 const bool sees = (anc_s[t] >> j) & 1;
                 const float ratio = __builtin_amdgcn_exp2f((float)(g_s[t] - gj) * kLog2e);
                 const float dot = (acc[0][e] + acc[1][e]) * (1.0f / (1 << (2 * kSplitExp)));
@@ -546,25 +609,29 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
     }
     // (the rows' z, for step 7)
     const size_t width = (size_t)p.value_heads * kW;
-    float z0[2 * RT], z1[2 * RT];
+    uint2 z[2 * RT];
 #pragma unroll
     for (int i = 0; i < 2 * RT; ++i) {
-        const size_t at = (size_t)(m.row0 + min(wave + 8 * i, R - 1)) * width + h * kW + lane;
-        z0[i] = load_act_nb(p.z, at, bf16);
-        z1[i] = load_act_nb(p.z, at + 64, bf16);
+        const size_t at = (size_t)(m.row0 + min(wave + 8 * i, R - 1)) * width + h * kW + 2 * lane;
+        if (bf16) z[i] = make_uint2(*(const uint32_t *)((const uint16_t *)p.z + at), 0);
+        else z[i] = *(const uint2 *)((const float *)p.z + at);
     }
     __syncthreads();
     // 5. column l16 of the inverse per lane
     if (wave < rt) {
         float *Ab = As + 16 * wave * kPair + 16 * wave;
+        f32x4 n[16][4];
+#pragma unroll
+        for (int t = 1; t < 16; ++t)
+#pragma unroll
+            for (int i = 0; i < (t + 3) / 4; ++i) n[t][i] = *(const f32x4 *)(Ab + t * kPair + 4 * i);
         float x[16];
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
-            float acc = (uint32_t)t == l16 ? 1.0f : 0.0f;
+        for (int t = 0; t < 16; ++t) x[t] = (uint32_t)t == l16 ? 1.0f : 0.0f;
 #pragma unroll
-            for (int i = 0; i < t; ++i) acc = fmaf(Ab[t * kPair + i], x[i], acc);
-            x[t] = acc;
-        }
+        for (int i = 0; i < 15; ++i)
+#pragma unroll
+            for (int t = i + 1; t < 16; ++t) x[t] = fmaf(n[t][i / 4][i % 4], x[i], x[t]);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         if (lane < 16) {
@@ -579,7 +646,7 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
 #pragma unroll
     for (int b = 0; b < RT; ++b) {
         if ((uint32_t)b >= rt) break;
-        float *vr = xv + (kHist + 16 * b + 4 * g4) * kPitch + 16 * wave + l16;
+        float *vr = xv + (16 * b + 4 * g4) * kPitch + 16 * wave + l16;
         f32x4 rhs, o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -606,21 +673,20 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
     __syncthreads();
     // 7. RMSNorm without offset, then * silu(z) (native.rs:737-740); rows past the
     // wave's last repeat it
-    const float n0 = p.norm[lane], n1 = p.norm[lane + 64];
+    const float n0 = p.norm[2 * lane], n1 = p.norm[2 * lane + 1];
     constexpr int kOut = 2 * RT < 4 ? 2 * RT : 4;  // rows at a time
 #pragma unroll
     for (int i0 = 0; i0 < 2 * RT; i0 += kOut) {
         if (wave + 8 * i0 >= R) break;
-        float o0[kOut], o1[kOut], inv[kOut];
+        float2 o[kOut];
+        float inv[kOut];
 #pragma unroll
         for (int i = 0; i < kOut; ++i) {
-            const float *o = xv + (kHist + min(wave + 8 * (i0 + i), R - 1)) * kPitch;
-            o0[i] = o[lane];
-            o1[i] = o[lane + 64];
+            o[i] = *(const float2 *)(xv + min(wave + 8 * (i0 + i), R - 1) * kPitch + 2 * lane);
         }
 #pragma unroll
         for (int i = 0; i < kOut; ++i) {
-            const float variance = wave_sum(fmaf(o1[i], o1[i], o0[i] * o0[i])) / (float)kW;
+            const float variance = wave_sum(fmaf(o[i].y, o[i].y, o[i].x * o[i].x)) / (float)kW;
             if (!isfinite(variance) && lane == 0) atomicOr(p.err_word, kErrNonFiniteVariance);
             inv[i] = 1.0f / sqrtf(variance + p.eps);
         }
@@ -628,9 +694,10 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
         for (int i = 0; i < kOut; ++i) {
             const uint32_t t = wave + 8 * (i0 + i);
             if (t >= R) break;
-            float *dst = p.out + (size_t)(m.row0 + t) * width + h * kW;
-            dst[lane] = o0[i] * inv[i] * n0 * silu_fast(z0[i0 + i]);
-            dst[lane + 64] = o1[i] * inv[i] * n1 * silu_fast(z1[i0 + i]);
+            const uint2 zi = z[i0 + i];
+            const float z0 = bf16 ? bf16lo(zi.x) : __uint_as_float(zi.x), z1 = bf16 ? bf16hi(zi.x) : __uint_as_float(zi.y);
+            *(float2 *)(p.out + (size_t)(m.row0 + t) * width + h * kW + 2 * lane) =
+                make_float2(o[i].x * inv[i] * n0 * silu_fast(z0), o[i].y * inv[i] * n1 * silu_fast(z1));
         }
     }
 }
