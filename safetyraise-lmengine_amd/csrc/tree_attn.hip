@@ -414,7 +414,11 @@ struct TreeShape {
     static constexpr int kThreads = 64 * NW;
     static constexpr int QP = kF32 ? 3 : 2;     // bf16 parts of q
     static constexpr int PP = kF32 ? 3 : 1;     // of the probabilities
-    static constexpr size_t kLds = kStages * kStageBytes + kTreePageSlots * 4;
+    // steps whose last part of q is kept in LDS, where the registers do not hold it: a
+    // spilled register's reload would wait for the stages on their way
+    static constexpr int kFarSteps = !kF32 ? 0 : D == 128 && VG == 4 ? 4 : D == 256 && VG == 1 ? 16 : 0;
+    static constexpr size_t kFarAt = kStages * kStageBytes + kTreePageSlots * 4;
+    static constexpr size_t kLds = kFarAt + VG * kFarSteps * 1024;
 };
 
 __device__ __forceinline__ float half_max(float x) {
@@ -502,13 +506,21 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
     const uint32_t vec = min(tile * 32 + col, nvec - 1);
     const uint32_t row = vec / group;  // of the sequence
     bf16x8 q[T::QP][NS];
+    unsigned char *far = lds + T::kFarAt + vg * (T::kFarSteps * 1024) + lane * 16;
     {
         const u32x4 *src = (const u32x4 *)c.q_ops +
                            (m.tile0 + (size_t)kvh * tiles + min(tile, tiles - 1)) * T::QP * NS * 64 + lane;
 #pragma unroll
         for (int p = 0; p < T::QP; ++p)
 #pragma unroll
-            for (int st = 0; st < NS; ++st) q[p][st] = __builtin_bit_cast(bf16x8, src[(p * NS + st) * 64]);
+            for (int st = 0; st < NS; ++st) {
+                if (p < T::QP - 1 || st < NS - T::kFarSteps) q[p][st] = __builtin_bit_cast(bf16x8, src[(p * NS + st) * 64]);
+            }
+        if constexpr (T::kFarSteps > 0) {
+            for (int st = (int)kg; st < T::kFarSteps; st += T::KG) {
+                *(u32x4 *)(far + st * 1024) = src[((T::QP - 1) * NS + NS - T::kFarSteps + st) * 64];
+            }
+        }
     }
     uint4 mask = c.masks[m.row0 + row];
 
@@ -521,7 +533,9 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
 #pragma unroll
     for (int p = 0; p < T::QP; ++p)
 #pragma unroll
-        for (int st = 0; st < NS; ++st) asm volatile("" : "+v"(q[p][st]));  // arrived
+        for (int st = 0; st < NS; ++st) {
+            if (p < T::QP - 1 || st < NS - T::kFarSteps) asm volatile("" : "+v"(q[p][st]));  // arrived
+        }
     asm volatile("" : "+v"(mask.x), "+v"(mask.y), "+v"(mask.z), "+v"(mask.w));
     const uint64_t mask_lo = ((uint64_t)mask.y << 32) | mask.x, mask_hi = ((uint64_t)mask.w << 32) | mask.z;
     __syncthreads();
@@ -605,7 +619,9 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
 #pragma unroll
             for (int p = 0; p < T::QP; ++p) {
                 f32x16 &x = acc[(st + p) % kChains];
-                x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[p][st], x, 0, 0, 0);
+                const bool near = p < T::QP - 1 || st < NS - T::kFarSteps;
+                const bf16x8 b = near ? q[p][st] : *(const bf16x8 *)(far + (st - (NS - T::kFarSteps)) * 1024);
+                x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, x, 0, 0, 0);
             }
         }
     };
@@ -639,7 +655,7 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
         // kLazy (or at the first visible key): sums and outputs are the same for any
         // common shift, and rescaling is rare.  (The maximum is of differences: of
         // the matrix products themselves it would cost a canonicalisation each.)
-        float ref = m_run == -INFINITY ? 0.0f : m_run;
+        const float ref = m_run == -INFINITY ? 0.0f : m_run;
         float d[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) d[i] = held[i] - ref;
@@ -653,7 +669,7 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
             const float scale = move ? __builtin_amdgcn_exp2f(m_run - next) : 1.0f;
             const bool summed = move && m_run > -INFINITY;  // (else there is nothing yet to rescale)
             m_run = next;
-            ref = next == -INFINITY ? 0.0f : next;
+            const float moved = next == -INFINITY ? 0.0f : next - ref;
             l_run *= scale;
             if (__builtin_amdgcn_ballot_w64(summed) == 0) {
                 // o is 0
@@ -679,8 +695,9 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[t][i] *= scale;
             }
+            // (from the differences: the scores' registers are free by now)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) d[i] = held[i] - ref;
+            for (int i = 0; i < 16; ++i) d[i] -= moved;
         }
         // V rows of the wave's keys: lane (i, h) reads its dims of keys 16 st + 4 h +
         // {0..3, 8..11}, those of its probabilities
