@@ -432,14 +432,23 @@ struct TreeLaunch {
     void *q_ops = nullptr, *masks = nullptr;  // scratch (tree_scratch)
     float *records = nullptr;
 };
+// How a launch is cut (tree_plan.hpp).
+struct TreePlan {
+    uint32_t vector_waves;  // waves of 32 query vectors per workgroup: 1, 2 or 4
+    uint64_t budget;        // of a partition: its keys times tree_key_cost
+    uint32_t max_part;      // keys of a partition at most
+    bool direct;            // one partition per sequence: no records
+    uint64_t record_bytes;
+};
 struct TreeScratch {
     size_t q_bytes = 0, mask_bytes = 0, record_bytes = 0;
+    TreePlan plan{};
 };
 constexpr uint32_t kTreeLaunchSeqs = 32, kTreeLaunchRows = 1024;
 TreeScratch tree_scratch(const TreeLaunch &a, const SeqMeta *seqs, int nseq, uint64_t call_rows,
                          int num_cus);
 hipError_t launch_tree_attn(hipStream_t stream, const TreeLaunch &a, const SeqMeta *seqs, int nseq,
-                            const uint8_t *parents, int num_cus);
+                            const uint8_t *parents, const TreePlan &plan);
 
 struct GdnLaunch {
     const safetyraise_kernel_gdn_pool *pool;

@@ -167,21 +167,23 @@ int32_t tree_forward(Ctx *ctx, const safetyraise_kernel_attention_tree_args *arg
     // share the scratch one after another
     struct Pack {
         uint32_t first, count;
+        TreePlan plan;
     };
     std::vector<Pack> packs;
     uint32_t pack_rows = 0;
     for (uint32_t i = 0; i < A.num_seqs; ++i) {
         if (packs.empty() || packs.back().count == kTreeLaunchSeqs ||
             pack_rows + seqs[i].rows > kTreeLaunchRows) {
-            packs.push_back({i, 0});
+            packs.push_back({i, 0, {}});
             pack_rows = 0;
         }
         ++packs.back().count;
         pack_rows += seqs[i].rows;
     }
     TreeScratch most;
-    for (const Pack &p : packs) {
+    for (Pack &p : packs) {
         const TreeScratch t = tree_scratch(L, &seqs[p.first], (int)p.count, total, ctx->num_cus);
+        p.plan = t.plan;
         most.q_bytes = std::max(most.q_bytes, t.q_bytes);
         most.mask_bytes = std::max(most.mask_bytes, t.mask_bytes);
         most.record_bytes = std::max(most.record_bytes, t.record_bytes);
@@ -221,7 +223,7 @@ int32_t tree_forward(Ctx *ctx, const safetyraise_kernel_attention_tree_args *arg
             }
         }
         const hipError_t e = launch_tree_attn(ctx->stream, L, &seqs[p.first], (int)p.count,
-                                              parents.data(), ctx->num_cus);
+                                              parents.data(), p.plan);
         if (e != hipSuccess) return hip_fail(ctx, e, "tree attention launch");
         L.tbl_n = 0;
     }

@@ -55,7 +55,7 @@ struct TreeCommon {
     uint64_t num_pages;
     uint32_t pages_per_seq, log2_page;
     uint32_t flags, heads, kv_heads, head_dim;
-    uint32_t nseq, part_keys;
+    uint32_t nseq;
     alignas(16) TreeMeta meta[kTreeSeqs];
 };
 
@@ -492,8 +492,9 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
     const uint32_t slice = (at - unit0 * slices) / width;
     const uint32_t kvh = unit % c.kv_heads;
     const uint32_t part = unit / c.kv_heads;
-    const uint32_t key_begin = part * c.part_keys;
-    const uint32_t key_end = min(key_begin + c.part_keys, m.ctx + m.rows);  // > key_begin
+    const uint32_t part_keys = tree_part_keys(m.ctx + m.rows, m.parts, D);
+    const uint32_t key_begin = part * part_keys;
+    const uint32_t key_end = min(key_begin + part_keys, m.ctx + m.rows);  // > key_begin
     const uint32_t steps = (key_end - key_begin + T::kKeys - 1) / T::kKeys;
 
     // this wave's query vectors (a wave without any only loads keys).  They are
@@ -924,12 +925,13 @@ TreeScratch tree_scratch(const TreeLaunch &a, const SeqMeta *seqs, int nseq, uin
     }
     const size_t parts = (a.flags & SAFETYRAISE_MI355X_OUTPUT_BF16) ? 2 : 3;
     t.q_bytes = tiles * 32 * a.head_dim * 2 * parts;
-    t.record_bytes = tree_plan(a.heads, a.kv_heads, a.head_dim, a.pool->page_tokens, num_cus, seqs, nseq).record_bytes;
+    t.plan = tree_plan(a.heads, a.kv_heads, a.head_dim, a.pool->page_tokens, num_cus, seqs, nseq);
+    t.record_bytes = t.plan.record_bytes;
     return t;
 }
 
 hipError_t launch_tree_attn(hipStream_t stream, const TreeLaunch &a, const SeqMeta *seqs, int nseq,
-                            const uint8_t *parents, int num_cus) {
+                            const uint8_t *parents, const TreePlan &plan) {
     PrepParams p{};
     TreeCommon &c = p.c;
     const auto *pool = a.pool;
@@ -957,10 +959,7 @@ hipError_t launch_tree_attn(hipStream_t stream, const TreeLaunch &a, const SeqMe
     c.kv_heads = a.kv_heads;
     c.head_dim = D;
     c.nseq = (uint32_t)nseq;
-    TreePlan plan{};
     if (!generic) {
-        plan = tree_plan(a.heads, a.kv_heads, D, pool->page_tokens, num_cus, seqs, nseq);
-        c.part_keys = plan.part_keys;
         c.records = plan.direct ? nullptr : a.records;
         if (!plan.direct && a.records == nullptr) return hipErrorInvalidValue;
     }
@@ -977,7 +976,7 @@ hipError_t launch_tree_attn(hipStream_t stream, const TreeLaunch &a, const SeqMe
         if (generic) continue;
         m.block0 = blocks;
         m.record0 = records;
-        m.parts = (m.ctx + m.rows + plan.part_keys - 1) / plan.part_keys;
+        m.parts = tree_parts(plan, D, m.ctx + m.rows, m.rows * group);
         const uint32_t per = plan.vector_waves * kTreeVectors;
         blocks += m.parts * a.kv_heads * ((m.rows * group + per - 1) / per);
         records += m.parts * m.rows * a.heads;

@@ -37,20 +37,38 @@ constexpr uint32_t tree_vector_waves(uint32_t head_dim) { return head_dim == 64 
 // LDS entries for the page ids of one partition.
 constexpr uint32_t kTreePageSlots = 1024;
 
-struct TreePlan {
-    uint32_t vector_waves;  // waves of 32 query vectors per workgroup: 1, 2 or 4
-    uint32_t part_keys;     // keys per partition, a multiple of the stage
-    bool direct;            // one partition per sequence: no records
-    uint64_t record_bytes;
-};
-
 // Bytes of a partition's record of one query vector: max, sum, 2 unused, o.
 constexpr uint32_t tree_record_floats(uint32_t head_dim) { return head_dim + 4; }
 
-// A workgroup fills its CU and costs its keys plus a start and end worth
-// kEnds keys; the merge of records costs kMerge.  The candidates are the
-// partitions that make one to four rounds of workgroups over the CUs, and one
-// partition per sequence.
+// Partitions of a sequence are equal: its keys over their number, up to whole stages.
+constexpr uint32_t tree_part_keys(uint32_t keys, uint32_t parts, uint32_t head_dim) {
+    const uint32_t stage = tree_stage_keys(head_dim);
+    return ((keys + parts - 1) / parts + stage - 1) / stage * stage;
+}
+
+// Time of a key in tenths: one where every SIMD has two waves with query vectors.  With
+// fewer vectors it has one, which waits for itself: 1.7 against 2.45 us per stage at
+// head width 128.
+inline uint32_t tree_key_cost(uint32_t head_dim, uint32_t vector_waves, uint64_t vectors) {
+    const uint32_t key_waves = tree_stage_keys(head_dim) / 32;
+    const uint64_t tiles = std::min<uint64_t>(vector_waves, (vectors + kTreeVectors - 1) / kTreeVectors);
+    return tiles * key_waves > 4 ? 10 : vector_waves * key_waves > 4 ? 7 : 10;
+}
+
+// The number of partitions of a sequence of `keys` (with the call's rows).
+inline uint32_t tree_parts(const TreePlan &plan, uint32_t head_dim, uint32_t keys, uint64_t vectors) {
+    const uint64_t stage = tree_stage_keys(head_dim);
+    uint64_t part = plan.budget / tree_key_cost(head_dim, plan.vector_waves, vectors) / stage * stage;
+    part = std::min<uint64_t>(std::max(part, stage), plan.max_part);
+    const uint64_t parts = (keys + part - 1) / part;
+    // (equal partitions of whole stages may be fewer)
+    const uint64_t equal = tree_part_keys(keys, (uint32_t)parts, head_dim);
+    return (uint32_t)((keys + equal - 1) / equal);
+}
+
+// A workgroup fills its CU and costs its keys plus a start and end worth kEnds keys; the
+// merge of records costs kMerge.  The candidates are the least budgets that make one to
+// four rounds of workgroups over the CUs, and one partition per sequence.
 inline TreePlan tree_plan(uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                           uint32_t page_tokens, int num_cus, const SeqMeta *seqs, int nseq) {
     const uint64_t stage = tree_stage_keys(head_dim);
@@ -58,54 +76,64 @@ inline TreePlan tree_plan(uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
     const uint64_t group = heads / kv_heads;
     auto up = [](uint64_t x, uint64_t unit) { return (x + unit - 1) / unit; };
     TreePlan plan{};
-    uint64_t most_vectors = 0, longest = 0;
-    for (int i = 0; i < nseq; ++i) {
-        most_vectors = std::max<uint64_t>(most_vectors, seqs[i].rows * group);
-        longest = std::max<uint64_t>(longest, (uint64_t)seqs[i].ctx + seqs[i].rows);
-    }
+    uint64_t most_vectors = 0, longest = 0, dearest = 0;
+    for (int i = 0; i < nseq; ++i) most_vectors = std::max<uint64_t>(most_vectors, seqs[i].rows * group);
     plan.vector_waves = 1;
     while (plan.vector_waves < tree_vector_waves(head_dim) &&
            plan.vector_waves * kTreeVectors < most_vectors) {
         plan.vector_waves *= 2;
     }
+    // (a partition that starts inside a page touches part / page + 2 pages)
+    plan.max_part = (uint32_t)((uint64_t)(kTreePageSlots - 2) * page_tokens / stage * stage);
     const uint64_t per_group = (uint64_t)plan.vector_waves * kTreeVectors;
-    auto blocks = [&](uint64_t part) {
+    for (int i = 0; i < nseq; ++i) {
+        const uint64_t keys = (uint64_t)seqs[i].ctx + seqs[i].rows;
+        longest = std::max(longest, keys);
+        dearest = std::max(dearest, up(keys, stage) * stage * tree_key_cost(head_dim, plan.vector_waves, seqs[i].rows * group));
+    }
+    auto blocks = [&](uint64_t budget) {
+        TreePlan p = plan;
+        p.budget = budget;
         uint64_t n = 0;
         for (int i = 0; i < nseq; ++i) {
-            n += up((uint64_t)seqs[i].ctx + seqs[i].rows, part) * up(seqs[i].rows * group, per_group);
+            const uint64_t vectors = seqs[i].rows * group;
+            n += tree_parts(p, head_dim, seqs[i].ctx + seqs[i].rows, vectors) * up(vectors, per_group);
         }
         return n * kv_heads;
     };
-    // (a partition that starts inside a page touches part / page + 2 pages)
-    const uint64_t max_part = (uint64_t)(kTreePageSlots - 2) * page_tokens / stage * stage;
-    const uint64_t whole = up(longest, stage) * stage;
-    constexpr uint64_t kEnds = 384, kMerge = 256;
+    constexpr uint64_t kEnds = 3840, kMerge = 2560;  // (tenths of a key)
+    const bool may_whole = up(longest, stage) * stage <= plan.max_part;
     uint64_t best = 0, best_time = ~0ull;
-    if (whole <= max_part) {
-        best = whole;
-        best_time = up(blocks(whole), cus) * (whole + kEnds);
+    if (may_whole) {
+        // (costs in tenths differ between sequences: with `dearest * 2` none is cut)
+        best = dearest * 2;
+        best_time = up(blocks(best), cus) * (dearest + kEnds);
     }
     for (uint64_t rounds = 1; rounds <= 4; ++rounds) {
-        uint64_t part = 4 * stage;
-        while (part < std::min(whole, max_part) && blocks(part) > rounds * cus) {
-            part += std::max<uint64_t>(stage, part / 16 / stage * stage);
+        uint64_t lo = 4 * stage * 10, hi = std::max(lo, dearest);  // (to 1 part in 256)
+        const uint64_t step = std::max(stage, (hi - lo) / 256);
+        if (blocks(lo) <= rounds * cus) hi = lo;
+        while (hi - lo > step) {
+            const uint64_t mid = (lo + hi) / 2;
+            if (blocks(mid) > rounds * cus) lo = mid;
+            else hi = mid;
         }
-        part = std::min(part, max_part);
-        const uint64_t time = up(blocks(part), cus) * (part + kEnds) + kMerge;
-        if (part < whole && time < best_time) {
+        const uint64_t time = up(blocks(hi), cus) * (hi + kEnds) + kMerge;
+        if (time < best_time) {
             best_time = time;
-            best = part;
+            best = hi;
         }
+        if (hi == 4 * stage * 10) break;  // more rounds make the same partitions
     }
-    plan.part_keys = (uint32_t)best;
-    plan.direct = best >= whole;
-    if (!plan.direct) {
-        uint64_t records = 0;
-        for (int i = 0; i < nseq; ++i) {
-            records += up((uint64_t)seqs[i].ctx + seqs[i].rows, best) * seqs[i].rows * heads;
-        }
-        plan.record_bytes = records * tree_record_floats(head_dim) * sizeof(float);
+    plan.budget = best;
+    uint64_t records = 0;
+    plan.direct = true;
+    for (int i = 0; i < nseq; ++i) {
+        const uint32_t parts = tree_parts(plan, head_dim, seqs[i].ctx + seqs[i].rows, seqs[i].rows * group);
+        plan.direct = plan.direct && parts == 1;
+        records += (uint64_t)parts * seqs[i].rows * heads;
     }
+    if (!plan.direct) plan.record_bytes = records * tree_record_floats(head_dim) * sizeof(float);
     return plan;
 }
 

@@ -35,7 +35,13 @@ static int tree() {
         sr::SeqMeta m[64] = {};
         for (unsigned i = 0; i < n; ++i) if (scanf("%u %u", &m[i].ctx, &m[i].rows) != 2) return 1;
         const sr::TreePlan p = sr::tree_plan(heads, kv, dim, page, 256, m, (int)n);
-        printf("%u %u %d %llu\n", p.vector_waves, p.part_keys, (int)p.direct, (unsigned long long)p.record_bytes);
+        printf("%u %d %llu", p.vector_waves, (int)p.direct, (unsigned long long)p.record_bytes);
+        for (unsigned i = 0; i < n; ++i) {
+            const unsigned keys = m[i].ctx + m[i].rows;
+            const unsigned parts = sr::tree_parts(p, dim, keys, m[i].rows * (heads / kv));
+            printf(" %u %u", parts, sr::tree_part_keys(keys, parts, dim));
+        }
+        printf("\n");
     }
     return 0;
 }
@@ -150,14 +156,14 @@ def test_tree_plans(ask):
                       [(rng.choice([0, 5, 300, 5000, rng.randint(0, 1 << 17)]), rng.randint(1, 128)) for _ in range(n)]))
     answers = ask("tree", [f"{h} {kv} {d} {p} {len(s)} " + " ".join(f"{c} {r}" for c, r in s)
                            for h, kv, d, p, s in calls])
-    for (heads, kv, dim, page, seqs), (waves, part, direct, record_bytes) in zip(calls, answers):
+    for (heads, kv, dim, page, seqs), (waves, direct, record_bytes, *parts) in zip(calls, answers):
         stage = 8192 // dim
-        assert part % stage == 0 and part > 0
         assert waves in (1, 2, 4) and waves <= (2 if dim == 64 else 4)
-        assert part // page + 2 <= 1024  # the partition's page ids fit in LDS
-        longest = max(c + r for c, r in seqs)
-        assert bool(direct) == (part >= longest)
-        want = 0 if direct else sum(-(-(c + r) // part) * r for c, r in seqs) * heads * (dim + 4) * 4
+        for (context, rows), n, part in zip(seqs, parts[::2], parts[1::2]):
+            assert part % stage == 0 and (n - 1) * part < context + rows <= n * part
+            assert part // page + 2 <= 1024  # the partition's page ids fit in LDS
+        assert bool(direct) == (max(parts[::2]) == 1)
+        want = 0 if direct else sum(n * r for n, (_, r) in zip(parts[::2], seqs)) * heads * (dim + 4) * 4
         assert record_bytes == want
 
 
