@@ -242,9 +242,13 @@ struct HeadShape {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-// (the records' rows are aligned to 4 bytes only)
+// (a caller's tensors may begin at any of their values, and a record's rows are aligned
+// to 4 bytes)
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
+typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2u __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32u __attribute__((aligned(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -321,8 +325,8 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
     uint32_t a_raw = 0, b_raw = 0, up_raw = 0;
     float a_log = 0.0f, dt_bias = 0.0f;
     if (wave == 0) {
-        a_raw = ((const uint32_t *)p.a)[bf16 ? ab_at >> 1 : ab_at];
-        b_raw = ((const uint32_t *)p.b)[bf16 ? ab_at >> 1 : ab_at];
+        a_raw = bf16 ? ((const uint16_t *)p.a)[ab_at] : ((const uint32_t *)p.a)[ab_at];
+        b_raw = bf16 ? ((const uint16_t *)p.b)[ab_at] : ((const uint32_t *)p.b)[ab_at];
         // (a lane's loads: scalar ones would be waited for here)
         uint32_t at = h;
         asm volatile("" : "+v"(at));
@@ -338,10 +342,10 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
     };
     if (bf16) {
 #pragma unroll
-        for (int n = 0; n < 3 * RT; ++n) raw16[n] = *(const u32x2 *)((const uint16_t *)p.qkv + raw_at(n));
+        for (int n = 0; n < 3 * RT; ++n) raw16[n] = *(const u32x2u *)((const uint16_t *)p.qkv + raw_at(n));
     } else {
 #pragma unroll
-        for (int n = 0; n < 3 * RT; ++n) raw[n] = *(const u32x4 *)((const float *)p.qkv + raw_at(n));
+        for (int n = 0; n < 3 * RT; ++n) raw[n] = *(const u32x4u *)((const float *)p.qkv + raw_at(n));
     }
     // the channels' history, one per thread
     const uint32_t hc = tid & 127, hpart = min(tid >> 7, 2u);
@@ -386,10 +390,8 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
     __builtin_amdgcn_sched_barrier(0);
     if (wave == 0) {
         // (used from here on: earlier, the compiler would wait for them before the other loads)
-        asm volatile("" : "+v"(up_raw), "+v"(a_log), "+v"(dt_bias));
-        const bool high = bf16 && (ab_at & 1);
-        const float av = !bf16 ? __uint_as_float(a_raw) : high ? bf16hi(a_raw) : bf16lo(a_raw);
-        const float bv = !bf16 ? __uint_as_float(b_raw) : high ? bf16hi(b_raw) : bf16lo(b_raw);
+        asm volatile("" : "+v"(a_raw), "+v"(b_raw), "+v"(up_raw), "+v"(a_log), "+v"(dt_bias));
+        const float av = __uint_as_float(bf16 ? a_raw << 16 : a_raw), bv = __uint_as_float(bf16 ? b_raw << 16 : b_raw);
         const int up = (int)up_raw - 1;
         const float log_a = -expf(a_log) * softplus_ref(av + dt_bias);
         // the path's set and sum up to, not with, `next`: doubling
@@ -609,12 +611,12 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
     }
     // (the rows' z, for step 7)
     const size_t width = (size_t)p.value_heads * kW;
-    uint2 z[2 * RT];
+    u32x2 z[2 * RT];
 #pragma unroll
     for (int i = 0; i < 2 * RT; ++i) {
         const size_t at = (size_t)(m.row0 + min(wave + 8 * i, R - 1)) * width + h * kW + 2 * lane;
-        if (bf16) z[i] = make_uint2(*(const uint32_t *)((const uint16_t *)p.z + at), 0);
-        else z[i] = *(const uint2 *)((const float *)p.z + at);
+        if (bf16) z[i].x = *(const u32u *)((const uint16_t *)p.z + at);
+        else z[i] = *(const u32x2u *)((const float *)p.z + at);
     }
     __syncthreads();
     // 5. column l16 of the inverse per lane
@@ -694,10 +696,10 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
         for (int i = 0; i < kOut; ++i) {
             const uint32_t t = wave + 8 * (i0 + i);
             if (t >= R) break;
-            const uint2 zi = z[i0 + i];
+            const u32x2 zi = z[i0 + i];
             const float z0 = bf16 ? bf16lo(zi.x) : __uint_as_float(zi.x), z1 = bf16 ? bf16hi(zi.x) : __uint_as_float(zi.y);
-            *(float2 *)(p.out + (size_t)(m.row0 + t) * width + h * kW + 2 * lane) =
-                make_float2(o[i].x * inv[i] * n0 * silu_fast(z0), o[i].y * inv[i] * n1 * silu_fast(z1));
+            *(f32x2u *)(p.out + (size_t)(m.row0 + t) * width + h * kW + 2 * lane) =
+                f32x2u{o[i].x * inv[i] * n0 * silu_fast(z0), o[i].y * inv[i] * n1 * silu_fast(z1)};
         }
     }
 }

@@ -46,9 +46,16 @@ class Case:
             np.log(1 + (decay - 1) * rng.random(hv)), np.log(np.expm1(step)),
             rng.standard_normal((self.channels, conv)) / 2, 1 + 0.1 * rng.standard_normal(dv))]
 
-    def run(self, asynchronous=False):
+    def run(self, asynchronous=False, offset=0):
+        def put(t):
+            if not self.device:
+                return t.numpy()
+            # (a tensor that begins `offset` values behind an aligned address)
+            whole = torch.empty(t.numel() + offset, dtype=t.dtype, device="cuda")
+            whole[offset:].copy_(t.reshape(-1))
+            return whole[offset:].view(t.shape)
+
         out = torch.full((self.rows, self.hv * self.dv), math.nan)
-        put = (lambda t: t.cuda()) if self.device else (lambda t: t.numpy())
         self.sent = [put(t) for t in self.inputs + self.weights]
         out = put(out)
         pkg.gdn_tree_forward(self.backend, self.pool, self.ids, [len(t) for t in self.trees],
@@ -131,6 +138,22 @@ def test_rows(backend, rows, depth):
     assert close(got, want)
     pkg.gdn_tree_commit(backend, [(case.pool, 0, rows - 1)])
     case.check_state(0, after[0][rows - 1])
+    case.pool.destroy()
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3])
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("widths", [(2, 4, 128, 128, 4), (1, 3, 128, 128, 3), (2, 2, 96, 40, 3)])
+def test_tensors_that_begin_anywhere(backend, widths, bf16, offset):
+    """Device tensors at any of their values' addresses."""
+    rng = np.random.default_rng(offset)
+    case = Case(backend, 9, *widths, [random_tree(rng, n)[0] for n in (21, 1, 5)], bf16=bf16)
+    got = case.run(offset=offset)
+    want, after = case.exact()
+    assert close(got, want)
+    pkg.gdn_tree_commit(backend, [(case.pool, i, 0) for i in case.ids])
+    for i in range(3):
+        case.check_state(i, after[i][0])
     case.pool.destroy()
 
 

@@ -9,8 +9,9 @@ does not widen the bound of the outputs.
 Bound of an output, with A = sum p |v| / sum p and S the largest sum |q k| /
 sqrt(D) of a visible key: q carries 32 roundings of 2^-24 (norm, RoPE, scale)
 and its parts 2^-24 (f32 out) or 2^-16; a score's sum D more: dS; a weight is
-off by 2 dS (its own and the sum's) and by its parts, 2^-16 (f32 out) or 2^-8;
-n weights are summed.
+off by 2 dS (its own and the sum's) and by its parts and the exponential, together
+2^-22 (f32 out: 2^-24 and a unit in the last place, 2^-23) or 2^-8; n weights are
+summed.
 """
 import importlib
 import math
@@ -149,7 +150,7 @@ class Case:
                     want, mag = p @ vv, p @ np.abs(vv)
                     big = (np.abs(kk) @ np.abs(q[at + r, h])).max() / math.sqrt(self.dim)
                     ds = big * ((32 + self.dim) * 2.0 ** -24 + (2.0 ** -16 if self.out16 else 2.0 ** -24))
-                    tol = mag * (2 * ds + (2.0 ** -8 if self.out16 else 2.0 ** -16) +
+                    tol = mag * (2 * ds + (2.0 ** -8 if self.out16 else 2.0 ** -22) +
                                  (len(see) + 64) * 2.0 ** -24)
                     if gate is not None:
                         g = 1 / (1 + np.exp(-gate[at + r, h]))
