@@ -376,9 +376,9 @@ SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_forward(
  * the caller gives the position of its depth in `positions`, and keeps the
  * accepted path with kv_compact.  At most MAX_TREE_ROWS rows per sequence.
  * out is f32, or bf16 with OUTPUT_BF16.  An f32 result carries f32 products
- * (q in three bf16 parts, probabilities in two, f32 sums); for a bf16 result
- * q is used in two parts and the probabilities in one, roundings below its
- * own.  Any head_dim 1..512 and any group of query heads; 64, 128 and 256
+ * (q and the probabilities in three bf16 parts each, f32 sums); for a bf16
+ * result q is used in two parts and the probabilities in one, roundings below
+ * its own.  Any head_dim 1..512 and any group of query heads; 64, 128 and 256
  * take the MFMA kernel. */
 typedef struct safetyraise_kernel_attention_tree_args {
     uint32_t struct_size;

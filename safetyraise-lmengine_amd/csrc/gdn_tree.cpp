@@ -287,6 +287,8 @@ SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_view(
     safetyraise_kernel_context *context, safetyraise_kernel_gdn_pool *pool, uint32_t sequence,
     const float **out_matrix, const float **out_history) {
     if (context == nullptr) return kInvalid;
+    const int32_t capture = refuse_under_capture(context, "gdn_view");
+    if (capture != kOk) return capture;
     if (pool == nullptr || out_matrix == nullptr || out_history == nullptr) {
         return fail(context, kInvalid, "NULL argument");
     }

@@ -309,7 +309,7 @@ def test_refusals(backend, change, text):
     case.pool.destroy()
 
 
-def test_refuses_too_many_rows_and_capture(backend):
+def test_refuses_too_many_rows(backend):
     case = Case(backend, 2, 4, 2, 64, 64, [list(range(-1, 127))], [0])
     big = torch.zeros((129, 4 * 64), device="cuda")
     pos = torch.zeros((129, 3), dtype=torch.int32, device="cuda")

@@ -159,3 +159,56 @@ def test_a_fork_keeps_other_tokens(backend):
     pool.append(a, k[:5], v[:5])
     assert np.array_equal(pool.read(0)[0], whole) and np.array_equal(pool.read(b)[0], kept_b)
     model.destroy()
+
+
+def test_capture_is_refused(backend):
+    """Every call refuses while the context's stream captures, and changes nothing."""
+    model = Layers(backend, 1, [20], attention=1, gdn=1)
+    kv, gdn = model.kv[0], model.gdn[0]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    inputs = inputs_of(g, 3)
+    torch.cuda.synchronize()
+    model.verify([[-1, 0, 0]], inputs)
+    backend.synchronize()
+    state = gdn.read(0)
+    k, v = (torch.zeros((2, KVH * DIM), device="cuda") for _ in range(2))
+    x = torch.zeros(4, device="cuda")
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    q, nk, nv = inputs[0][0]
+    pos = torch.zeros((3, 3), dtype=torch.int32, device="cuda")
+    out, gout = torch.zeros((3, HEADS * DIM), device="cuda"), torch.zeros((3, HV * DV), device="cuda")
+    calls = [
+        lambda: pkg.attention_tree_forward(backend, kv, [0], [3], [-1, 0, 0], q, nk, nv, pos, out, heads=HEADS,
+                                           kv_heads=KVH, head_dim=DIM, rotary_dim=DIM, rope_theta=1e6,
+                                           asynchronous=True),
+        lambda: pkg.gdn_tree_forward(backend, gdn, [0], [3], [-1, 0, 0], *inputs[1][0], *model.weights[0], gout,
+                                     asynchronous=True),
+        lambda: pkg.gdn_tree_commit(backend, [(gdn, 0, 1)], asynchronous=True),
+        lambda: pkg.kv_compact(backend, [(kv, 0, 0, 20, [1])], asynchronous=True),
+        lambda: pkg.kv_gather(backend, [(kv, 0, 0, 2)], k, v, asynchronous=True),
+        lambda: gdn.view(0),
+    ]
+    texts = []
+    torch.cuda.synchronize()
+    backend.set_stream(stream.cuda_stream)
+    try:
+        with torch.cuda.graph(graph, stream=stream):
+            x.add_(1.0)
+            for call in calls:
+                try:
+                    call()
+                    texts.append("ran")
+                except pkg.PluginError as e:
+                    texts.append(str(e))
+    finally:
+        backend.set_stream(None)
+    assert all("cannot be captured" in t for t in texts), texts
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(x, torch.ones(4, device="cuda"))
+    assert kv.len(0) == 23 and np.array_equal(gdn.read(0)[0], state[0])
+    for call in calls:  # outside capture the same calls run
+        call()
+        backend.synchronize()
+    assert kv.len(0) == 21
+    model.destroy()
