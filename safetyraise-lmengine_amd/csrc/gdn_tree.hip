@@ -207,15 +207,16 @@ __global__ void __launch_bounds__(256) gdn_tree_generic_kernel(const GdnTreePara
 // Dk = Dv = 128: one workgroup of 8 waves per (value head, sequence), everything
 // between the inputs and the outputs in LDS and registers.
 //
-// Wave w owns state rows 16 w .. 16 w + 15 (32 registers, requested first) and
-// the same columns of every [row][Dv] matrix:
-//   1. raw conv inputs to LDS behind the history; decays, ancestors, conv taps
-//      (one wave, pointer doubling over the parents)
-//   2. conv + silu in place, last row first (a row reads rows before it)
-//   3. q and k normalised, as fp16 parts
-//   4. K S0^T and Q S0^T per wave; K K^T and Q K^T blocks over the waves, masked
-//      and decayed:  A[t][j] = -b_t e^{g_t - g_j} (k^_t . k^_j),  j above t
-//                    P[t][j] = e^{g_t - g_j} (q^_t . k^_j),       j above or t
+// Wave w owns state rows 16 w .. 16 w + 15 (32 registers, requested with the inputs)
+// and the same columns of every [row][Dv] matrix:
+//   1. raw conv inputs to LDS behind the history, 16 bytes per lane; decays, ancestors,
+//      conv taps (one wave, pointer doubling over the parents)
+//   2. v, q, k in turn: conv + silu of a row, two channels per lane, into memory that
+//      no row reads any more;
+//   3. with them q and k normalised, as fp16 parts
+//   4. K S0^T and Q S0^T per wave; on the way K K^T and Q K^T blocks, masked and
+//      decayed:  A[t][j] = -b_t e^{g_t - g_j} (k^_t . k^_j),  j above t
+//                P[t][j] = e^{g_t - g_j} (q^_t . k^_j),       j above or t
 //   5. T = (I - A_bb)^-1 of each 16-row block
 //   6. block by block  D_b = T_b (b_t (V - e^{g_t} K^ S0^T) + sum_{c<b} A_bc D_c),
 //      O_b = e^{g_t} Q^ S0^T + sum_{c<=b} P_bc D_c
@@ -223,6 +224,14 @@ __global__ void __launch_bounds__(256) gdn_tree_generic_kernel(const GdnTreePara
 // The products of step 6 are v_mfma_f32_16x16x4_f32 with 4 consecutive k per lane; an
 // accumulator (rows 4 g + i of lane group g) is the next product's B operand as it is.
 // RT: 16-row tiles of the longest tree.
+//
+// What bounds it: the chain of phases, each bound by something else.  Eight sequences of
+// 24..64 rows, 16 key and 32 value heads: 28.7 us for 40 MB (8.3 us at the copy rate):
+// inputs and state 7, conv and norms 6.3 (vector instructions: exponentials and
+// reciprocals of the silu; q and k are made once per value head of theirs), products 4.9,
+// solve 0.7, step 6 2.2, outputs 1.6.  One sequence of 12 rows: 10.6 us, mostly latency and
+// the fetch of the code.  With 4-byte loads, the conv in place and the norms in a pass
+// of their own it took 32 us.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kW = 128;         // Dk and Dv
 constexpr uint32_t kPitch = kW + 4;  // floats per LDS row (16 rows of 16 bytes meet no bank twice)
@@ -723,11 +732,13 @@ struct CommitParams {
 };
 static_assert(sizeof(CommitParams) <= 4096, "kernel arguments stay within 4 KiB");
 
-constexpr uint32_t kCommitRows = 4;  // state rows per thread
+constexpr uint32_t kCommitRows = 8;  // state rows per thread
 
 // S = a S + d k^T along the path: 16-byte units of the state, a thread the same
 // columns of kCommitRows rows, then the conv channels' last K - 1 inputs.  grid
-// (blocks of the largest entry, entries)
+// (blocks of the largest entry, entries).  Bound by the state's bytes: 8 layers of 4
+// sequences with 32 heads of 128 x 128, 144 MB: 28 us, 5.1 TB/s; the rows of a thread
+// share a path row's k (four rows: 29.5 us, one: 42).
 template <typename Unit>
 __global__ void __launch_bounds__(256) gdn_tree_commit_kernel(const CommitParams p) {
     constexpr uint32_t W = sizeof(Unit) / 4;

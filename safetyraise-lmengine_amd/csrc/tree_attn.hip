@@ -98,8 +98,10 @@ __device__ __forceinline__ TreeMeta find_meta(const TreeCommon &c, uint32_t r) {
                     get(x.x, at + 1), get(x.y, at + 1), get(x.z, at + 1), get(x.w, at + 1)};
 }
 
-// One wave per (row, four heads): KV heads first, then query heads.  NI: dims
-// per lane, d = lane + 64 i.
+// One wave per (row, head): KV heads first, then query heads.  NI: dims per lane,
+// d = lane + 64 i.  Bound by latency: arguments, inputs, one exchange through LDS, and
+// the fetch of its code, so that heads are waves and not a loop unrolled (4.5 us for 6
+// rows of 16 heads; four heads per wave took 7.8).
 template <uint32_t NI>
 __global__ void __launch_bounds__(256) tree_prep_kernel(const PrepParams p) {
     extern __shared__ float xs_all[];
@@ -391,13 +393,24 @@ __global__ void __launch_bounds__(64) tree_generic_kernel(const TreeCommon c) {
 // is one query vector, so its maximum takes one exchange between the two halves
 // of the wave, and the probabilities are in the layout of the next product's
 // operand where they are made.  q and p are split into bf16 parts that sum to
-// them (kF32: 24 bits of q, 16 of p; else 16 and 8), products and sums are f32.
+// them: three of each (24 bits) for an f32 result; for a bf16 result two of q (its
+// rounding is multiplied by the scores' size) and one of p, whose rounding is no
+// larger than the result's own.  Products and sums are f32.
 //
 // A workgroup has up to 4 x 32 query vectors and 32 KB stages of kKeys keys: a
 // wave takes one of the vector groups and 32 keys of a stage.  Stages come
 // straight into LDS (global_load_lds, 16 bytes per lane), kAhead ahead, one
-// barrier per stage; a row's 16-byte units are swapped by its index so that the
-// operand reads (ds_read_b128 of K, ds_read_b64_tr_b16 of V) meet no bank twice.
+// barrier per stage.  K rows have their 16-byte units swapped by the row's index, so
+// that the operand reads (ds_read_b128) meet no bank twice; V rows are read as they
+// are, a lane the same D / 32 dims of 8 keys, and v_perm_b32 pairs the keys' values
+// for the product.  The scores of stage k run beside the softmax and P V of stage
+// k - 1.
+//
+// What bounds it: the matrix pipe.  Eight sequences of 16..32 rows behind 1024..16384
+// tokens, 32 heads over 8 of width 128, f32: 120 us, of which 89 are its products at the
+// 1205 TFLOP/s that a large bf16 matrix product reaches, and 79 the loads alone.  Four
+// of 20..64 rows behind 8192..65536 tokens at width 256, bf16: 245 us; products 184, loads 74.
+// The rest is mostly waits for LDS at width 256, where a wave has a SIMD to itself.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kStages = 4;
 constexpr uint32_t kAhead = 2;  // stages on their way; one more may still be read by late waves
@@ -831,7 +844,7 @@ __global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_
 }
 
 // Joins the records of a (row, head): a wave each, all the loads of eight records
-// in flight.
+// in flight.  Bound by the records' bytes (32 MB in 8.9 us at width 256).
 template <int D>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeCommon c, uint32_t rows) {
     constexpr int EPL = D / 64, kBatch = 8;
