@@ -77,13 +77,40 @@ struct Words {
     }
 };
 
+// Whether all tokens are below the limit (> 0).  The sign of t | (limit - 1 - t) says so for
+// a limit up to 2^31, in operations of every vector unit.
+bool all_below(const uint32_t *tokens, uint64_t count, uint64_t limit) {
+    uint32_t bad = 0;
+    if (limit <= 1ull << 31) {
+        const uint32_t top = (uint32_t)limit - 1;
+        for (uint64_t j = 0; j < count; ++j) bad |= tokens[j] | (top - tokens[j]);
+        return bad >> 31 == 0;
+    }
+    for (uint64_t j = 0; j < count; ++j) bad |= tokens[j] >= limit ? 1u : 0u;
+    return bad == 0;
+}
+
+bool all_ascend(const uint32_t *tokens, uint64_t count) {
+    if (count == 0) return true;
+    uint32_t bad = 0, high = tokens[0];
+    for (uint64_t j = 1; j < count; ++j) {
+        bad |= tokens[j] - tokens[j - 1] - 1;
+        high |= tokens[j];
+    }
+    if (high >> 31 == 0) return bad >> 31 == 0;
+    for (uint64_t j = 1; j < count; ++j) {
+        if (tokens[j] <= tokens[j - 1]) return false;
+    }
+    return true;
+}
+
 // Token lists of a call by address: layers usually share them.
 struct Lists {
     struct One {
         const uint32_t *tokens;
         uint64_t count;
-        uint32_t limit;  // all tokens are below it
-        bool ascending;
+        uint64_t below;   // all tokens are below it (0: not looked at)
+        bool ascending;   // (likewise)
         uint32_t offset;  // in the words; 0: not yet
     };
     std::vector<One> lists;
@@ -94,12 +121,21 @@ struct Lists {
         for (size_t i = lists.size(); i-- > 0 && i + 32 > lists.size();) {
             if (lists[i].tokens == tokens && lists[i].count == count) return (uint32_t)i;
         }
-        uint32_t most = 0;
-        bool ascending = true;
-        for (uint64_t j = 0; j < count; ++j) most = std::max(most, tokens[j]);
-        for (uint64_t j = 1; j < count; ++j) ascending &= tokens[j] > tokens[j - 1];
-        lists.push_back({tokens, count, count == 0 ? 0 : most + 1, ascending && most != UINT32_MAX, 0});
+        lists.push_back({tokens, count, 0, false, 0});
         return (uint32_t)lists.size() - 1;
+    }
+    bool below(uint32_t i, uint64_t limit) {
+        One &l = lists[i];
+        if (l.below != 0 && l.below <= limit) return true;
+        if (limit == 0 || !all_below(l.tokens, l.count, limit)) return false;
+        l.below = limit;
+        return true;
+    }
+    // ascending strictly, and below the limit
+    bool ascend_below(uint32_t i, uint64_t limit) {
+        One &l = lists[i];
+        l.ascending = l.ascending || all_ascend(l.tokens, l.count);
+        return l.ascending && l.tokens[l.count - 1] < limit;
     }
 };
 
@@ -136,8 +172,7 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
         }
         if (e.count > 0) {
             list_of[i] = lists.add(e.tokens, e.count);
-            const Lists::One &l = lists.lists[list_of[i]];
-            if (!l.ascending || l.limit > source.len - e.start) {
+            if (!lists.ascend_below(list_of[i], source.len - e.start)) {
                 return fail(ctx, kInvalid,
                             "kv_compact tokens must ascend strictly and stay within the sequence");
             }
@@ -344,8 +379,7 @@ int32_t gather(Ctx *ctx, const safetyraise_kernel_kv_rows *entries, uint32_t n, 
         bool inside = e.start <= len && (e.tokens != nullptr || e.count <= len - e.start);
         if (inside && e.tokens != nullptr && e.count > 0) {
             list_of[i] = lists.add(e.tokens, e.count);
-            const uint64_t limit = lists.lists[list_of[i]].limit;
-            inside = limit != 0 && limit <= len - e.start;  // (0: a token of 2^32 - 1)
+            inside = lists.below(list_of[i], len - e.start);
         }
         if (!inside) return fail(ctx, kInvalid, "KV token index out of range");
         total += e.count;

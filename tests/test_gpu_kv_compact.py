@@ -1,5 +1,6 @@
 """kv_compact and kv_gather against lists of rows on the host: copies, so every
 comparison is for equality."""
+import ctypes as C
 import importlib
 
 import numpy as np
@@ -292,6 +293,33 @@ def test_refusals(backend):
     for bad in ((a, 0, [50]), (a, 51, 0), (a, 49, 2)):
         with pytest.raises(pkg.PluginError, match="out of range"):
             pkg.kv_gather(backend, [(m.pool, *bad)], k, k.clone())
+    m.pool.destroy()
+
+
+@pytest.mark.parametrize("token", [50, 2 ** 31 - 1, 2 ** 31, 2 ** 31 + 1, 2 ** 32 - 1])
+@pytest.mark.parametrize("at", [0, 7, 20])
+def test_tokens_out_of_range(backend, token, at):
+    """One token too large, anywhere in a list, in every place of a vector."""
+    m = Model(backend, np.random.default_rng(1))
+    a, b = m.new(50), m.new(20)
+    good = list(range(20))
+    k, v = (np.zeros((21, m.width), np.float32) for _ in range(2))
+    with pytest.raises(pkg.PluginError, match="out of range"):
+        pkg.kv_gather(backend, [(m.pool, a, 0, good[:at] + [token] + good[at:])], k, v)
+    for tokens in (good[:at] + [token], good[:at] + [token] + [x + 21 for x in good[at:]], [5, 5], [9, 8, 10]):
+        with pytest.raises(pkg.PluginError, match="ascend strictly"):
+            pkg.kv_compact(backend, [(m.pool, a, b, 0, tokens)])
+        m.check()
+    # a list that two entries share: within one sequence, beyond the other
+    shared = (C.c_uint32 * 21)(*range(21))
+    k, v = (np.zeros((42, m.width), np.float32) for _ in range(2))
+    for order, status in (((a, b), 1), ((b, a), 1), ((a, a), 0)):
+        entries = (pkg.plugin.KvRows * 2)()
+        for e, sequence in zip(entries, order):
+            e.kv, e.sequence, e.count, e.tokens = m.pool.handle, sequence, 21, shared
+        assert status == backend.lib.safetyraise_kernel_kv_gather(
+            backend.context, entries, 2, k.ctypes.data, v.ctypes.data, 0)
+    assert np.array_equal(k, np.concatenate([m.held[a][0][:21]] * 2))
     m.pool.destroy()
 
 
