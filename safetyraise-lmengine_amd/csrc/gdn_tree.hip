@@ -737,9 +737,11 @@ constexpr uint32_t kCommitRows = 8;  // state rows per thread
 // S = a S + d k^T along the path: 16-byte units of the state, a thread the same
 // columns of kCommitRows rows, then the conv channels' last K - 1 inputs.  grid
 // (blocks of the largest entry, entries).  Bound by the state's bytes: 8 layers of 4
-// sequences with 32 heads of 128 x 128, 144 MB: 28 us, 5.1 TB/s; the rows of a thread
-// share a path row's k (four rows: 29.5 us, one: 42).
-template <typename Unit>
+// sequences with 32 heads of 128 x 128, 144 MB: 30 us with inputs of its own each call,
+// 4.8 TB/s, the rate of a copy (37.5 through the caches).  The rows of a thread share a
+// path row's k (eight rows 28.1 us, four 29.5, one 41.7, sixteen 31.3, all with the
+// state still in the last cache).
+template <typename Unit, typename Unaligned>
 __global__ void __launch_bounds__(256) gdn_tree_commit_kernel(const CommitParams p) {
     constexpr uint32_t W = sizeof(Unit) / 4;
     const GdnCommitEntry e = p.entries != nullptr ? p.entries[blockIdx.y] : p.inline_entries[blockIdx.y];
@@ -753,32 +755,39 @@ __global__ void __launch_bounds__(256) gdn_tree_commit_kernel(const CommitParams
         const uint32_t c = (uint32_t)(u % per);
         const uint32_t band = (uint32_t)(u / per % bands), h = (uint32_t)(u / per / bands);
         const uint32_t kh = h / (e.value_heads / e.key_heads);
-        alignas(16) float S[kCommitRows][W];
+        const float *state_in = global_from_bits<const float>((uint64_t)e.state_in);
+        float *state_out = global_from_bits<float>((uint64_t)e.state_out);
+        const float *records = global_from_bits<const float>((uint64_t)e.records);
+        // (read and written once each: past the caches)
+        Unit S[kCommitRows];
         uint32_t v[kCommitRows];
 #pragma unroll
         for (uint32_t i = 0; i < kCommitRows; ++i) {
             v[i] = min(band + bands * i, e.value_dim - 1);
-            *(Unit *)S[i] = *((const Unit *)(e.state_in + ((size_t)h * e.value_dim + v[i]) * e.key_dim) + c);
+            S[i] = __builtin_nontemporal_load((const Unit *)(state_in + ((size_t)h * e.value_dim + v[i]) * e.key_dim) + c);
         }
         for (uint64_t path = e.path; path != 0; path &= path - 1) {
-            const float *rec = e.records + (size_t)__builtin_ctzll(path) * e.rec_stride;
+            const float *rec = records + (size_t)__builtin_ctzll(path) * e.rec_stride;
             const float alpha = rec[h];
-            float k[W];
-            const float *key = rec + e.value_heads * (1 + e.value_dim) + kh * e.key_dim + W * c;
+            const Unit k = *(const Unaligned *)(rec + e.value_heads * (1 + e.value_dim) + kh * e.key_dim + W * c);
+            float delta[kCommitRows];
 #pragma unroll
-            for (uint32_t j = 0; j < W; ++j) k[j] = key[j];
+            for (uint32_t i = 0; i < kCommitRows; ++i) delta[i] = rec[e.value_heads + h * e.value_dim + v[i]];
 #pragma unroll
             for (uint32_t i = 0; i < kCommitRows; ++i) {
-                const float delta = rec[e.value_heads + h * e.value_dim + v[i]];
+                if constexpr (W == 1) {
+                    S[i] = fmaf(delta[i], k, S[i] * alpha);
+                } else {
 #pragma unroll
-                for (uint32_t j = 0; j < W; ++j) S[i][j] = fmaf(delta, k[j], S[i][j] * alpha);
+                    for (uint32_t j = 0; j < W; ++j) S[i][j] = fmaf(delta[i], k[j], S[i][j] * alpha);
+                }
             }
         }
 #pragma unroll
         for (uint32_t i = 0; i < kCommitRows; ++i) {
             // (rows past the last repeat it)
             if (band + bands * i < e.value_dim) {
-                *((Unit *)(e.state_out + ((size_t)h * e.value_dim + v[i]) * e.key_dim) + c) = *(const Unit *)S[i];
+                __builtin_nontemporal_store(S[i], (Unit *)(state_out + ((size_t)h * e.value_dim + v[i]) * e.key_dim) + c);
             }
         }
         return;
@@ -882,10 +891,10 @@ hipError_t launch_gdn_tree_commit(hipStream_t stream, const GdnCommitEntry *entr
         }
     }
     if (vec) {
-        SR_LAUNCH("gdn_tree_commit_kernel", gdn_tree_commit_kernel<float4>, dim3((uint32_t)blocks[0], count),
+        SR_LAUNCH("gdn_tree_commit_kernel", (gdn_tree_commit_kernel<f32x4, f32x4u>), dim3((uint32_t)blocks[0], count),
                   dim3(256), 0, stream, p);
     } else {
-        SR_LAUNCH("gdn_tree_commit_kernel", gdn_tree_commit_kernel<float>, dim3((uint32_t)blocks[1], count),
+        SR_LAUNCH("gdn_tree_commit_kernel", (gdn_tree_commit_kernel<float, float>), dim3((uint32_t)blocks[1], count),
                   dim3(256), 0, stream, p);
     }
     return hipGetLastError();

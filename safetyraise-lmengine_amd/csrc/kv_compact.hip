@@ -1,11 +1,13 @@
 // Tokens moved inside a KV pool and copied out of it, for lists of tokens of many
 // sequences and pools in one launch.
 //
-// Both are copies: bound by the bytes they read and write (14500 of 53000 tokens of
-// two sequences, 8 heads of width 128, to free pages, 119 MB: 24 us, 5 TB/s; 33300 of
-// three, 2 heads of width 256, to f32 rows, 205 MB: 37.5 us, 5.5 TB/s), or for a few tokens by the launch (4.6 us).  The call's description (entries, ranges, token lists, page
-// ids) travels in the kernel arguments where it fits, else through pinned host
-// memory into a device buffer.
+// Both are copies: bound by the bytes they read and write, or for a few tokens by the
+// launch (4.6 us).  14500 of 53000 tokens of two sequences, 8 heads of width 128, to free
+// pages, 119 MB: 24 us; 33300 of three, 2 heads of width 256, to f32 rows, 205 MB: 37.5 us
+// where the last cache holds part of it, 43 where not.
+//
+// The call's description (entries, ranges, token lists, page ids) travels in the
+// kernel arguments where it fits, else through pinned host memory into a device buffer.
 #include "kv_moves.hpp"
 #include "sr_device.hpp"
 
@@ -115,6 +117,20 @@ struct GatherArgs {
 };
 static_assert(sizeof(GatherArgs) <= 4096, "kernel arguments stay within 4 KiB");
 
+// Unit `at` of an output, past the caches: written once, and as a rule more than they
+// hold (205 MB: 58 us with plain stores, 47 with these, where each call has inputs and
+// outputs of its own).
+__device__ __forceinline__ void put8(void *out, size_t at, Unit16 x, bool bf16) {
+    typedef float Half __attribute__((ext_vector_type(4)));
+    if (bf16) {
+        __builtin_nontemporal_store(x, (Unit16 *)out + at);
+    } else {
+        Half *to = (Half *)out + 2 * at;
+        __builtin_nontemporal_store(Half{bf16lo(x.x), bf16hi(x.x), bf16lo(x.y), bf16hi(x.y)}, to);
+        __builtin_nontemporal_store(Half{bf16lo(x.z), bf16hi(x.z), bf16lo(x.w), bf16hi(x.w)}, to + 1);
+    }
+}
+
 // One workgroup per block of at most block_tokens tokens of one entry; a thread
 // takes 8 values (kVec) or one value of a token's K and V rows at a time.
 template <bool kVec>
@@ -154,16 +170,8 @@ __global__ void __launch_bounds__(256) kv_gather_rows_kernel(const GatherArgs a)
 #pragma unroll
             for (uint32_t u = 0; u < kBatch; ++u) {
                 if (!ok[u]) break;
-                if (a.bf16_out) {
-                    ((Unit16 *)a.keys)[dst[u]] = k[u];
-                    ((Unit16 *)a.values)[dst[u]] = v[u];
-                } else {
-                    float4 *dk = (float4 *)a.keys + 2 * dst[u], *dv = (float4 *)a.values + 2 * dst[u];
-                    dk[0] = make_float4(bf16lo(k[u].x), bf16hi(k[u].x), bf16lo(k[u].y), bf16hi(k[u].y));
-                    dk[1] = make_float4(bf16lo(k[u].z), bf16hi(k[u].z), bf16lo(k[u].w), bf16hi(k[u].w));
-                    dv[0] = make_float4(bf16lo(v[u].x), bf16hi(v[u].x), bf16lo(v[u].y), bf16hi(v[u].y));
-                    dv[1] = make_float4(bf16lo(v[u].z), bf16hi(v[u].z), bf16lo(v[u].w), bf16hi(v[u].w));
-                }
+                put8(a.keys, dst[u], k[u], a.bf16_out != 0);
+                put8(a.values, dst[u], v[u], a.bf16_out != 0);
             }
         } else {
 #pragma unroll
