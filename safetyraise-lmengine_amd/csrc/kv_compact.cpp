@@ -60,7 +60,7 @@ bool is_open(const Pool *pool, uint32_t seq) {
 
 // The words of a call: in the kernel arguments (`small`) or in an upload slot.
 struct Words {
-    uint32_t small[kMoveInlineWords];
+    alignas(16) uint32_t small[kMoveInlineWords];
     uint32_t *at = nullptr;
 
     int32_t open(Ctx *ctx, size_t count, size_t most_inline) {
