@@ -212,3 +212,61 @@ def test_capture_is_refused(backend):
         backend.synchronize()
     assert kv.len(0) == 21
     model.destroy()
+
+
+@pytest.mark.parametrize("dim,kvh", [(64, 16), (128, 8), (256, 4), (80, 13)])
+def test_cache_past_32_bits(backend, dim, kvh):
+    """A pool whose last heads begin past 2^31 values and 2^32 bytes gives the results of
+    a small one, bit for bit."""
+    pages = 2 ** 31 // ((kvh - 1) * 64 * dim) + 64
+    rng = np.random.default_rng(dim)
+    k, v = (rng.standard_normal((300, kvh * dim)).astype(np.float32) for _ in range(2))
+    tree = random_tree(rng, 20)[0]
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    q, nk, nv = (torch.randn(20, n * dim, device="cuda", generator=g) for n in (2 * kvh, kvh, kvh))
+    pos = torch.tensor([[300 + len(ancestors(tree, r)) - 1] * 3 for r in range(20)], dtype=torch.int32).cuda()
+    results = []
+    for n in (64, pages):
+        pool = pkg.KvCache(backend, kvh, dim, 64, n, 1024, 3, page_order_seed=n)
+        a, b = pool.open(), pool.open()
+        pool.append(a, k, v)
+        out = torch.zeros((20, 2 * kvh * dim), device="cuda")
+        torch.cuda.synchronize()
+        pkg.attention_tree_forward(backend, pool, [a], [20], tree, q, nk, nv, pos, out, heads=2 * kvh,
+                                   kv_heads=kvh, head_dim=dim, rotary_dim=dim, rope_theta=1e6)
+        pkg.kv_compact(backend, [(pool, a, b, 7, list(range(0, 313, 3)))])
+        pkg.kv_compact(backend, [(pool, a, a, 300, ancestors(tree, 19))])
+        rows = [np.zeros((pool.len(a) + pool.len(b), kvh * dim), np.float32) for _ in range(2)]
+        pkg.kv_gather(backend, [(pool, a, 0, pool.len(a)), (pool, b, 0, pool.len(b))], *rows)
+        results.append([out.cpu().numpy(), *rows])
+        pool.destroy()
+    for small, large in zip(*results):
+        assert np.array_equal(small, large)
+    assert np.array_equal(results[1][1][:300], torch.from_numpy(k).bfloat16().float().numpy())
+
+
+def test_states_past_32_bits(backend):
+    """The last sequences of a large pool of states and records."""
+    seqs = 1500
+    pool = pkg.GdnState(backend, 16, 32, 128, 128, 4, seqs, keep_rows=64)
+    ids = [pool.open() for _ in range(seqs)]
+    rng = np.random.default_rng(5)
+    m = 0.2 * rng.standard_normal((32, 128, 128)).astype(np.float32)
+    h = rng.standard_normal((8192, 3)).astype(np.float32)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    tree = random_tree(rng, 25)[0]
+    x = [torch.randn(25, n, device="cuda", generator=g) for n in (8192, 4096, 32, 32)]
+    w = [torch.rand(32, device="cuda", generator=g), torch.randn(32, device="cuda", generator=g) - 3,
+         torch.randn((8192, 4), device="cuda", generator=g) / 2, torch.ones(128, device="cuda")]
+    results = []
+    for i in (ids[0], ids[-1]):
+        pool.write(i, m, h)
+        out = torch.zeros((25, 4096), device="cuda")
+        torch.cuda.synchronize()
+        pkg.gdn_tree_forward(backend, pool, [i], [25], tree, *x, *w, out)
+        pkg.gdn_tree_commit(backend, [(pool, i, 24)])
+        results.append([out.cpu().numpy(), *pool.read(i)])
+    for first, last in zip(*results):
+        assert np.array_equal(first, last)
+    assert not np.array_equal(results[0][1], m)
+    pool.destroy()
