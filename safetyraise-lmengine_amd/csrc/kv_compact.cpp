@@ -246,7 +246,24 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
     int32_t st = w.open(ctx, words, kMoveInlineWords);
     if (st != kOk) return st;
 
-    // nothing fails from here on but a launch: the new page lists, and the words
+    std::vector<MoveLink> late;
+    std::vector<std::pair<Pool *, int32_t>> given_up;
+    std::vector<int32_t> now;
+    size_t most = 0, old_pages = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        const auto &e = entries[i];
+        const CompactPlan &p = known[plan_of[i]].plan;
+        auto &target = e.kv->seqs[e.target];
+        most = std::max(most, p.take.size());
+        if (e.target == e.source) old_pages += target.pages.size() - p.first;
+        target.pages.reserve(p.first + p.take.size());
+    }
+    late.reserve(n);
+    given_up.reserve(old_pages);
+    now.reserve(most);
+
+    // nothing fails from here on but a launch (and nothing is allocated: a pool's free
+    // list has room for all its pages): the new page lists, and the words
     for (uint32_t i = 0; i < n; ++i) {
         const auto &e = entries[i];
         if (e.target == e.source) continue;
@@ -260,10 +277,7 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
     MoveRange *head = (MoveRange *)(move + n), *tail = head + chains;
     MoveRange *const first_range = head;
     MoveLink *link = (MoveLink *)(head + ranges);
-    std::vector<MoveLink> late;
-    std::vector<std::pair<Pool *, int32_t>> given_up;
     uint32_t *list = w.at + fixed;
-    std::vector<int32_t> now;
     MoveCall call{};
     for (uint32_t i = 0; i < n; ++i, ++move) {
         const auto &e = entries[i];
