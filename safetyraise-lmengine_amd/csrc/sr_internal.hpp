@@ -434,7 +434,6 @@ struct TreeLaunch {
 };
 // How a launch is cut (tree_plan.hpp).
 struct TreePlan {
-    uint32_t vector_waves;  // waves of 32 query vectors per workgroup: 1, 2 or 4
     uint64_t budget;        // of a partition: its keys times tree_key_cost
     uint32_t max_part;      // keys of a partition at most
     bool direct;            // one partition per sequence: no records

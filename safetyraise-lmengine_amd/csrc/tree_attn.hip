@@ -419,8 +419,9 @@ constexpr float kLazy = 8.0f;  // log2 growth of the maximum before sums are res
 
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 
-template <int D, int VG, bool kF32>
+template <int D, bool kF32>
 struct TreeShape {
+    static constexpr int VG = (int)tree_vector_waves(D);  // waves of query vectors
     static constexpr int kKeys = 8192 / D;      // keys per stage
     static constexpr int KG = kKeys / 32;       // waves over the keys of a stage
     static constexpr int NW = VG * KG;
@@ -429,7 +430,7 @@ struct TreeShape {
     static constexpr int PP = kF32 ? 3 : 1;     // of the probabilities
     // steps whose last part of q is kept in LDS, where the registers do not hold it: a
     // spilled register's reload would wait for the stages on their way
-    static constexpr int kFarSteps = !kF32 ? 0 : D == 128 && VG == 4 ? 4 : D == 256 && VG == 1 ? 16 : 0;
+    static constexpr int kFarSteps = kF32 && D == 128 ? 4 : 0;
     static constexpr size_t kFarAt = kStages * kStageBytes + kTreePageSlots * 4;
     static constexpr size_t kLds = kFarAt + VG * kFarSteps * 1024;
 };
@@ -474,9 +475,10 @@ __device__ __forceinline__ bf16x8 v_operand(const VRow<NT> (&v)[8], int t) {
     return __builtin_bit_cast(bf16x8, x);
 }
 
-template <int D, int VG, bool kF32>
-__global__ __launch_bounds__((TreeShape<D, VG, kF32>::kThreads)) void tree_attn_kernel(const TreeCommon c) {
-    using T = TreeShape<D, VG, kF32>;
+template <int D, bool kF32>
+__global__ __launch_bounds__((TreeShape<D, kF32>::kThreads)) void tree_attn_kernel(const TreeCommon c) {
+    using T = TreeShape<D, kF32>;
+    constexpr int VG = T::VG;
     constexpr int NS = D / 16, NT = D / 32;
     constexpr int CH = D / 8;             // 16-byte units per row
     constexpr int RPI = 64 / CH;          // rows per load instruction
@@ -889,31 +891,24 @@ __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeCommon c, u
     }
 }
 
-template <int D, int VG, bool kF32>
+template <int D, bool kF32>
 hipError_t launch_attn(hipStream_t stream, const TreeCommon &c, uint32_t blocks) {
-    using T = TreeShape<D, VG, kF32>;
+    using T = TreeShape<D, kF32>;
     static_assert(T::kLds <= 160 * 1024, "LDS");
     static const hipError_t configured =
-        hipFuncSetAttribute((const void *)tree_attn_kernel<D, VG, kF32>,
+        hipFuncSetAttribute((const void *)tree_attn_kernel<D, kF32>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)T::kLds);
     if (configured != hipSuccess) return configured;
-    SR_LAUNCH("tree_attn_kernel", (tree_attn_kernel<D, VG, kF32>), dim3(blocks), dim3(T::kThreads),
+    SR_LAUNCH("tree_attn_kernel", (tree_attn_kernel<D, kF32>), dim3(blocks), dim3(T::kThreads),
               T::kLds, stream, c);
     return hipGetLastError();
 }
 
 template <int D>
-hipError_t launch_width(hipStream_t stream, const TreeCommon &c, uint32_t blocks, uint32_t rows,
-                        uint32_t vector_waves) {
-    const bool f32 = (c.flags & SAFETYRAISE_MI355X_OUTPUT_BF16) == 0;
-    hipError_t e = hipErrorInvalidValue;
-    if (vector_waves == 1) {
-        e = f32 ? launch_attn<D, 1, true>(stream, c, blocks) : launch_attn<D, 1, false>(stream, c, blocks);
-    } else if (vector_waves == 2) {
-        e = f32 ? launch_attn<D, 2, true>(stream, c, blocks) : launch_attn<D, 2, false>(stream, c, blocks);
-    } else if constexpr (tree_vector_waves(D) == 4) {
-        e = f32 ? launch_attn<D, 4, true>(stream, c, blocks) : launch_attn<D, 4, false>(stream, c, blocks);
-    }
+hipError_t launch_width(hipStream_t stream, const TreeCommon &c, uint32_t blocks, uint32_t rows) {
+    const hipError_t e = (c.flags & SAFETYRAISE_MI355X_OUTPUT_BF16) == 0
+                             ? launch_attn<D, true>(stream, c, blocks)
+                             : launch_attn<D, false>(stream, c, blocks);
     if (e != hipSuccess || c.records == nullptr) return e;
     SR_LAUNCH("tree_combine_kernel", tree_combine_kernel<D>, dim3((rows * c.heads + 3) / 4), dim3(256),
               0, stream, c, rows);
@@ -990,7 +985,7 @@ hipError_t launch_tree_attn(hipStream_t stream, const TreeLaunch &a, const SeqMe
         m.block0 = blocks;
         m.record0 = records;
         m.parts = tree_parts(plan, D, m.ctx + m.rows, m.rows * group);
-        const uint32_t per = plan.vector_waves * kTreeVectors;
+        const uint32_t per = tree_vector_waves(D) * kTreeVectors;
         blocks += m.parts * a.kv_heads * ((m.rows * group + per - 1) / per);
         records += m.parts * m.rows * a.heads;
     }
@@ -1023,9 +1018,9 @@ hipError_t launch_tree_attn(hipStream_t stream, const TreeLaunch &a, const SeqMe
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     switch (D) {
-        case 64: return launch_width<64>(stream, c, blocks, rows, plan.vector_waves);
-        case 128: return launch_width<128>(stream, c, blocks, rows, plan.vector_waves);
-        case 256: return launch_width<256>(stream, c, blocks, rows, plan.vector_waves);
+        case 64: return launch_width<64>(stream, c, blocks, rows);
+        case 128: return launch_width<128>(stream, c, blocks, rows);
+        case 256: return launch_width<256>(stream, c, blocks, rows);
         default: break;
     }
     SR_LAUNCH("tree_generic_kernel", tree_generic_kernel, dim3(a.heads, rows), dim3(64),

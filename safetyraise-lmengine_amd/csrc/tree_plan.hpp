@@ -31,7 +31,8 @@ inline uint64_t tree_path(const int32_t *parents, int32_t row) {
 // One stage of the tree kernel: 32 KB of K and V.
 constexpr uint32_t tree_stage_keys(uint32_t head_dim) { return 8192 / head_dim; }
 // Query vectors (rows x heads of a KV head) per wave, and waves of vectors per
-// workgroup at most.
+// workgroup: as many for few vectors too, as the waves without any still load keys (1..3
+// rows of 4 heads at width 128 behind 8192..20000 tokens: 69 us with four, 78 with one).
 constexpr uint32_t kTreeVectors = 32;
 constexpr uint32_t tree_vector_waves(uint32_t head_dim) { return head_dim == 64 ? 2 : 4; }
 // LDS entries for the page ids of one partition.
@@ -49,8 +50,8 @@ constexpr uint32_t tree_part_keys(uint32_t keys, uint32_t parts, uint32_t head_d
 // Time of a key in tenths: one where every SIMD has two waves with query vectors.  With
 // fewer vectors it has one, which waits for itself: 1.7 against 2.45 us per stage at
 // head width 128.
-inline uint32_t tree_key_cost(uint32_t head_dim, uint32_t vector_waves, uint64_t vectors) {
-    const uint32_t key_waves = tree_stage_keys(head_dim) / 32;
+inline uint32_t tree_key_cost(uint32_t head_dim, uint64_t vectors) {
+    const uint32_t key_waves = tree_stage_keys(head_dim) / 32, vector_waves = tree_vector_waves(head_dim);
     const uint64_t tiles = std::min<uint64_t>(vector_waves, (vectors + kTreeVectors - 1) / kTreeVectors);
     return tiles * key_waves > 4 ? 10 : vector_waves * key_waves > 4 ? 7 : 10;
 }
@@ -58,7 +59,7 @@ inline uint32_t tree_key_cost(uint32_t head_dim, uint32_t vector_waves, uint64_t
 // The number of partitions of a sequence of `keys` (with the call's rows).
 inline uint32_t tree_parts(const TreePlan &plan, uint32_t head_dim, uint32_t keys, uint64_t vectors) {
     const uint64_t stage = tree_stage_keys(head_dim);
-    uint64_t part = plan.budget / tree_key_cost(head_dim, plan.vector_waves, vectors) / stage * stage;
+    uint64_t part = plan.budget / tree_key_cost(head_dim, vectors) / stage * stage;
     part = std::min<uint64_t>(std::max(part, stage), plan.max_part);
     const uint64_t parts = (keys + part - 1) / part;
     // (equal partitions of whole stages may be fewer)
@@ -66,9 +67,12 @@ inline uint32_t tree_parts(const TreePlan &plan, uint32_t head_dim, uint32_t key
     return (uint32_t)((keys + equal - 1) / equal);
 }
 
-// A workgroup fills its CU and costs its keys plus a start and end worth kEnds keys; the
-// merge of records costs kMerge.  The candidates are the least budgets that make one to
-// four rounds of workgroups over the CUs, and one partition per sequence.
+// A workgroup fills its CU and costs its keys plus a start and an end, about 8 us; the
+// merge of records is 4.5 us and the writing and reading of them at 4 TB/s (17 / D^2 tenths
+// of a key per float).  A stage takes about D / 64 x 0.5 us (its products per wave go with
+// D), so that these are worth keys in inverse proportion to D^2: 300 tokens at width 256
+// take 21 us in partitions of two stages, 45 in one.  The candidates are the least budgets
+// that make one to four rounds of workgroups over the CUs, and one partition per sequence.
 inline TreePlan tree_plan(uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                           uint32_t page_tokens, int num_cus, const SeqMeta *seqs, int nseq) {
     const uint64_t stage = tree_stage_keys(head_dim);
@@ -76,63 +80,61 @@ inline TreePlan tree_plan(uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
     const uint64_t group = heads / kv_heads;
     auto up = [](uint64_t x, uint64_t unit) { return (x + unit - 1) / unit; };
     TreePlan plan{};
-    uint64_t most_vectors = 0, longest = 0, dearest = 0;
-    for (int i = 0; i < nseq; ++i) most_vectors = std::max<uint64_t>(most_vectors, seqs[i].rows * group);
-    plan.vector_waves = 1;
-    while (plan.vector_waves < tree_vector_waves(head_dim) &&
-           plan.vector_waves * kTreeVectors < most_vectors) {
-        plan.vector_waves *= 2;
-    }
+    uint64_t longest = 0, dearest = 0;
     // (a partition that starts inside a page touches part / page + 2 pages)
     plan.max_part = (uint32_t)((uint64_t)(kTreePageSlots - 2) * page_tokens / stage * stage);
-    const uint64_t per_group = (uint64_t)plan.vector_waves * kTreeVectors;
+    const uint64_t per_group = (uint64_t)tree_vector_waves(head_dim) * kTreeVectors;
     for (int i = 0; i < nseq; ++i) {
         const uint64_t keys = (uint64_t)seqs[i].ctx + seqs[i].rows;
         longest = std::max(longest, keys);
-        dearest = std::max(dearest, up(keys, stage) * stage * tree_key_cost(head_dim, plan.vector_waves, seqs[i].rows * group));
+        dearest = std::max(dearest, up(keys, stage) * stage * tree_key_cost(head_dim, seqs[i].rows * group));
     }
+    uint64_t records = 0;  // of the budget that blocks() last looked at
     auto blocks = [&](uint64_t budget) {
         TreePlan p = plan;
         p.budget = budget;
         uint64_t n = 0;
+        records = 0;
         for (int i = 0; i < nseq; ++i) {
             const uint64_t vectors = seqs[i].rows * group;
-            n += tree_parts(p, head_dim, seqs[i].ctx + seqs[i].rows, vectors) * up(vectors, per_group);
+            const uint64_t parts = tree_parts(p, head_dim, seqs[i].ctx + seqs[i].rows, vectors);
+            n += parts * up(vectors, per_group);
+            records += parts * seqs[i].rows * heads;
         }
         return n * kv_heads;
     };
-    constexpr uint64_t kEnds = 3840, kMerge = 2560;  // (tenths of a key)
+    const uint64_t square = (uint64_t)head_dim * head_dim;
+    const uint64_t ends = 20000 * 4096 / square, merge = 11000 * 4096 / square;  // (tenths of a key)
+    constexpr uint64_t kLeast = 2;  // stages of a partition
     const bool may_whole = up(longest, stage) * stage <= plan.max_part;
     uint64_t best = 0, best_time = ~0ull;
     if (may_whole) {
         // (costs in tenths differ between sequences: with `dearest * 2` none is cut)
         best = dearest * 2;
-        best_time = up(blocks(best), cus) * (dearest + kEnds);
+        best_time = up(blocks(best), cus) * (dearest + ends);
     }
     for (uint64_t rounds = 1; rounds <= 4; ++rounds) {
-        uint64_t lo = 4 * stage * 10, hi = std::max(lo, dearest);  // (to 1 part in 256)
-        const uint64_t step = std::max(stage, (hi - lo) / 256);
+        uint64_t lo = kLeast * stage * 10, hi = std::max(lo, dearest);  // (to 1 part in 1024)
+        const uint64_t step = std::max(stage, (hi - lo) / 1024);
         if (blocks(lo) <= rounds * cus) hi = lo;
         while (hi - lo > step) {
             const uint64_t mid = (lo + hi) / 2;
             if (blocks(mid) > rounds * cus) lo = mid;
             else hi = mid;
         }
-        const uint64_t time = up(blocks(hi), cus) * (hi + kEnds) + kMerge;
+        const uint64_t time = up(blocks(hi), cus) * (hi + ends) + merge +
+                              records * tree_record_floats(head_dim) * 17 / square;
         if (time < best_time) {
             best_time = time;
             best = hi;
         }
-        if (hi == 4 * stage * 10) break;  // more rounds make the same partitions
+        if (hi == kLeast * stage * 10) break;  // more rounds make the same partitions
     }
     plan.budget = best;
-    uint64_t records = 0;
-    plan.direct = true;
-    for (int i = 0; i < nseq; ++i) {
-        const uint32_t parts = tree_parts(plan, head_dim, seqs[i].ctx + seqs[i].rows, seqs[i].rows * group);
-        plan.direct = plan.direct && parts == 1;
-        records += (uint64_t)parts * seqs[i].rows * heads;
-    }
+    (void)blocks(best);
+    uint64_t rows = 0;
+    for (int i = 0; i < nseq; ++i) rows += seqs[i].rows;
+    plan.direct = records == rows * heads;
     if (!plan.direct) plan.record_bytes = records * tree_record_floats(head_dim) * sizeof(float);
     return plan;
 }

@@ -35,7 +35,7 @@ static int tree() {
         sr::SeqMeta m[64] = {};
         for (unsigned i = 0; i < n; ++i) if (scanf("%u %u", &m[i].ctx, &m[i].rows) != 2) return 1;
         const sr::TreePlan p = sr::tree_plan(heads, kv, dim, page, 256, m, (int)n);
-        printf("%u %d %llu", p.vector_waves, (int)p.direct, (unsigned long long)p.record_bytes);
+        printf("%d %llu", (int)p.direct, (unsigned long long)p.record_bytes);
         for (unsigned i = 0; i < n; ++i) {
             const unsigned keys = m[i].ctx + m[i].rows;
             const unsigned parts = sr::tree_parts(p, dim, keys, m[i].rows * (heads / kv));
@@ -156,9 +156,8 @@ def test_tree_plans(ask):
                       [(rng.choice([0, 5, 300, 5000, rng.randint(0, 1 << 17)]), rng.randint(1, 128)) for _ in range(n)]))
     answers = ask("tree", [f"{h} {kv} {d} {p} {len(s)} " + " ".join(f"{c} {r}" for c, r in s)
                            for h, kv, d, p, s in calls])
-    for (heads, kv, dim, page, seqs), (waves, direct, record_bytes, *parts) in zip(calls, answers):
+    for (heads, kv, dim, page, seqs), (direct, record_bytes, *parts) in zip(calls, answers):
         stage = 8192 // dim
-        assert waves in (1, 2, 4) and waves <= (2 if dim == 64 else 4)
         for (context, rows), n, part in zip(seqs, parts[::2], parts[1::2]):
             assert part % stage == 0 and (n - 1) * part < context + rows <= n * part
             assert part // page + 2 <= 1024  # the partition's page ids fit in LDS
