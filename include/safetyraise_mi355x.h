@@ -424,8 +424,9 @@ SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_tree_commit(
     uint32_t num_commits, uint32_t flags);
 
 /* Device addresses of a sequence's current state [Hv][Dv][Dk] and conv
- * history [C][K-1] (f32), valid until the next call that changes or closes
- * the sequence.  Work queued on the context's stream comes before them. */
+ * history [C][K-1] (f32).  What they hold is the sequence's until the next call
+ * that changes or closes it; gdn_destroy frees them, whoever still reads them.
+ * Work queued on the context's stream comes before them. */
 SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_view(
     safetyraise_kernel_context *context, safetyraise_kernel_gdn_pool *pool, uint32_t sequence,
     const float **out_matrix, const float **out_history);

@@ -672,10 +672,32 @@ def kv_gather(backend: NativeBackend, reads, keys, values, asynchronous: bool = 
         backend.context, entries, len(reads), _ptr(keys), _ptr(values), flags), "kv_gather")
 
 
-class _DeviceArray:
-    """f32 device memory for torch.as_tensor."""
+class _PoolMemory:
+    """A pool on the device, held by its GdnState and by every tensor on its memory:
+    freed when it has been given up (destroy) and the last of them is gone."""
 
-    def __init__(self, pointer: int, shape):
+    def __init__(self, backend: NativeBackend, handle):
+        self.backend, self.handle = backend, handle
+        self.given_up = False
+        self.viewed = None  # the device of the tensors on it, if there were any
+
+    def __del__(self):
+        if not self.given_up:
+            return
+        if self.viewed is not None:
+            # what reads it may still be queued on a stream of the caller's
+            import torch
+
+            torch.cuda.synchronize(self.viewed)
+        self.backend.lib.safetyraise_kernel_gdn_destroy(self.backend.context, self.handle)
+
+
+class _DeviceArray:
+    """f32 device memory for torch.as_tensor, which keeps this object as long as any
+    tensor is on the memory."""
+
+    def __init__(self, memory: _PoolMemory, pointer: int, shape):
+        self.memory = memory
         self.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": "<f4", "version": 2,
                                          "data": (pointer, False), "strides": None}
 
@@ -695,7 +717,12 @@ class GdnState:
         handle = C.c_void_p()
         backend.check(backend.lib.safetyraise_kernel_gdn_create(backend.context, C.byref(opts),
                                                                 C.byref(handle)), "gdn_create")
-        self.handle = handle
+        self._memory = _PoolMemory(backend, handle)
+
+    @property
+    def handle(self):
+        """The pool, or None after destroy."""
+        return self._memory.handle if self._memory is not None else None
 
     def _call(self, name: str, *args):
         fn = getattr(self.backend.lib, f"safetyraise_kernel_gdn_{name}")
@@ -727,24 +754,29 @@ class GdnState:
 
     def view(self, seq: int):
         """The current state [Hv][Dv][Dk] and history [C][K-1] as torch tensors on
-        the pool's own memory, valid until the sequence changes."""
+        the pool's own memory, which stays as long as they or tensors made on them
+        do, also after destroy.  Their values are the sequence's until its next call
+        that changes or closes it."""
         import torch
 
         matrix, history = C.c_void_p(), C.c_void_p()
         self._call("view", seq, C.byref(matrix), C.byref(history))
         shapes = ((self.value_heads, self.value_dim, self.key_dim),
                   (self.channels, self.conv_kernel - 1))
-        return tuple(torch.as_tensor(_DeviceArray(p.value, shape), device="cuda")
-                     for p, shape in zip((matrix, history), shapes))
+        views = tuple(torch.as_tensor(_DeviceArray(self._memory, p.value, shape), device="cuda")
+                      for p, shape in zip((matrix, history), shapes))
+        self._memory.viewed = views[0].device
+        return views
 
     def rollback(self, seq: int, rows: int, asynchronous: bool = False) -> None:
         """State and history after the first `rows` rows of the last KEEP_ROWS call."""
         self._call("rollback", seq, rows, ASYNC if asynchronous else 0)
 
     def destroy(self) -> None:
-        if self.handle is not None and self.handle.value:
-            self.backend.lib.safetyraise_kernel_gdn_destroy(self.backend.context, self.handle)
-            self.handle = None
+        """Frees the pool, or leaves that to the last tensor on its memory (view)."""
+        if self._memory is not None:
+            self._memory.given_up = True
+            self._memory = None
 
 
 def gdn_forward(backend: NativeBackend, state: GdnState, seq_ids: Sequence[int],
