@@ -347,6 +347,7 @@ class NativeBackend:
         self.context = C.c_void_p(context)
         self.name = name
         self.capabilities = caps
+        self.stream: Optional[int] = None  # set_stream's; None: the context's own
 
     @classmethod
     def load(cls, path: Optional[os.PathLike] = None) -> "NativeBackend":
@@ -450,6 +451,7 @@ class NativeBackend:
     def set_stream(self, stream_handle: Optional[int]) -> None:
         self.check(self.lib.safetyraise_kernel_set_stream(self.context, stream_handle),
                    "setting the stream")
+        self.stream = stream_handle
 
     def synchronize(self) -> None:
         self.check(self.lib.safetyraise_kernel_synchronize(self.context), "synchronizing")
@@ -702,6 +704,19 @@ class _DeviceArray:
                                          "data": (pointer, False), "strides": None}
 
 
+def _on_memory(array: _DeviceArray, devices):
+    """A torch tensor on the array's memory: torch.as_tensor copies to the device that
+    it is told, unless that is where the memory is."""
+    import torch
+
+    at = array.__cuda_array_interface__["data"][0]
+    for d in devices:
+        tensor = torch.as_tensor(array, device=f"cuda:{d}")
+        if tensor.data_ptr() == at or tensor.numel() == 0:
+            return tensor
+    raise RuntimeError("no device of torch has the pool's memory")
+
+
 class GdnState:
     """Per-sequence GDN recurrent state pool (RecurrentState per slot)."""
 
@@ -756,17 +771,29 @@ class GdnState:
         """The current state [Hv][Dv][Dk] and history [C][K-1] as torch tensors on
         the pool's own memory, which stays as long as they or tensors made on them
         do, also after destroy.  Their values are the sequence's until its next call
-        that changes or closes it."""
+        that changes or closes it.  The caller's current torch stream waits for the
+        calls that the context has queued; it may not be one that is captured."""
         import torch
 
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("gdn_view cannot be captured into a graph")
         matrix, history = C.c_void_p(), C.c_void_p()
         self._call("view", seq, C.byref(matrix), C.byref(history))
-        shapes = ((self.value_heads, self.value_dim, self.key_dim),
-                  (self.channels, self.conv_kernel - 1))
-        views = tuple(torch.as_tensor(_DeviceArray(self._memory, p.value, shape), device="cuda")
-                      for p, shape in zip((matrix, history), shapes))
-        self._memory.viewed = views[0].device
-        return views
+        first = torch.cuda.current_device()
+        devices = [first] + [d for d in range(torch.cuda.device_count()) if d != first]
+        state = _on_memory(_DeviceArray(self._memory, matrix.value, (
+            self.value_heads, self.value_dim, self.key_dim)), devices)
+        device = self._memory.viewed = state.device
+        history = _on_memory(_DeviceArray(self._memory, history.value, (
+            self.channels, self.conv_kernel - 1)), [device.index])
+        # (the default stream is behind the context's own one, which is a blocking one)
+        stream = torch.cuda.default_stream(device)
+        if self.backend.stream is not None:
+            stream = torch.cuda.ExternalStream(self.backend.stream, device=device)
+        current = torch.cuda.current_stream(device)
+        if current.cuda_stream != stream.cuda_stream:
+            current.wait_stream(stream)
+        return state, history
 
     def rollback(self, seq: int, rows: int, asynchronous: bool = False) -> None:
         """State and history after the first `rows` rows of the last KEEP_ROWS call."""

@@ -40,21 +40,45 @@ class HostArray:
         self.__array_interface__ = dict(array.__cuda_array_interface__, version=3)
 
 
+class Stream:
+    def __init__(self, log, handle):
+        self.log, self.cuda_stream = log, handle
+
+    def wait_stream(self, other):
+        self.log.append("stream %d waits for %d" % (self.cuda_stream, other.cuda_stream))
+
+
+class Tensor(torch.Tensor):
+    """A host tensor that says it is on a GPU."""
+    device = None
+
+
 @pytest.fixture
 def library(monkeypatch):
     lib = Library()
+    lib.home, lib.current, lib.stream, lib.capturing = 0, 0, 0, False
 
     def as_tensor(array, device=None):
-        lib.log.append("tensor")
-        return torch.from_numpy(np.asarray(HostArray(array)))
+        x = torch.from_numpy(np.asarray(HostArray(array)))
+        there = torch.device(device).index == lib.home
+        lib.log.append("tensor" if there else "copy")
+        x = (x if there else x.clone()).as_subclass(Tensor)
+        x.device = torch.device(device)
+        return x
 
     monkeypatch.setattr(torch, "as_tensor", as_tensor)
     monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: lib.log.append("synchronize"))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: lib.capturing)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: lib.current)
+    monkeypatch.setattr(torch.cuda, "device_count", lambda: 3)
+    monkeypatch.setattr(torch.cuda, "default_stream", lambda device=None: Stream(lib.log, 0))
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream(lib.log, lib.stream))
+    monkeypatch.setattr(torch.cuda, "ExternalStream", lambda handle, device=None: Stream(lib.log, handle))
     return lib
 
 
-def new_pool(lib):
-    backend = types.SimpleNamespace(lib=lib, context=1, check=lambda status, what: None)
+def new_pool(lib, stream=None):
+    backend = types.SimpleNamespace(lib=lib, context=1, stream=stream, check=lambda status, what: None)
     return pkg.GdnState(backend, 1, HV, DK, DV, TAPS + 1, 1, keep_rows=4)
 
 
@@ -108,3 +132,34 @@ def test_destroy_after_the_views(library):
     pool.destroy()
     assert handle.value == 77
     assert library.log[-2:] == ["synchronize", "destroy 77"]
+
+
+@pytest.mark.parametrize("current,context,want", [
+    (0, None, []),  # the default stream and a blocking one
+    (5, None, ["stream 5 waits for 0"]),
+    (5, 5, []),
+    (5, 9, ["stream 5 waits for 9"]),
+    (0, 9, ["stream 0 waits for 9"]),
+])
+def test_callers_stream_waits(library, current, context, want):
+    library.stream = current
+    new_pool(library, context).view(0)
+    assert [x for x in library.log if x.startswith("stream")] == want
+
+
+@pytest.mark.parametrize("home,current", [(0, 0), (2, 0), (1, 2)])
+def test_another_device_is_current(library, home, current):
+    """A view is on the pool's memory, not a copy on the current device."""
+    library.home, library.current = home, current
+    pool = new_pool(library)
+    state, history = pool.view(0)
+    assert state.device.index == history.device.index == home
+    assert state.data_ptr() == library.state.ctypes.data
+    assert history.data_ptr() == library.history.ctypes.data
+
+
+def test_no_view_under_capture(library):
+    library.capturing = True
+    with pytest.raises(RuntimeError, match="captured"):
+        new_pool(library).view(0)
+    assert "view" not in library.log

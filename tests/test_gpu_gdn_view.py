@@ -37,3 +37,43 @@ def test_view_outlives_the_pool(backend):
     assert np.array_equal(row.cpu().numpy(), held[1][0][2, 5])
     for other in others:
         other.destroy()
+
+
+@pytest.mark.parametrize("context_stream", [False, True])
+def test_view_on_another_stream(backend, context_stream):
+    """A view on a stream of the caller's is behind the asynchronous calls before it."""
+    pool, held = new_pool(backend, 4, sequences=8)
+    rng = np.random.default_rng(5)
+    rows, width = 8 * 8, 4 * 128
+    inputs = [torch.from_numpy(rng.standard_normal((rows, n)).astype(np.float32)).cuda()
+              for n in (pool.channels, width, 4, 4)]
+    weights = [torch.from_numpy(rng.standard_normal(n).astype(np.float32)).cuda()
+               for n in (4, 4, (pool.channels, 4), 128)]
+    out = torch.zeros((rows, width), device="cuda")
+    torch.cuda.synchronize()
+    contexts, side = torch.cuda.Stream(), torch.cuda.Stream()
+    if context_stream:
+        backend.set_stream(contexts.cuda_stream)
+    try:
+        for turn in range(20):
+            pkg.gdn_tree_forward(backend, pool, list(range(8)), [8] * 8, [-1, 0, 1, 1, 3, 4, 5, 6] * 8,
+                                 *inputs, *weights, out, asynchronous=True)
+            pkg.gdn_tree_commit(backend, [(pool, i, 7) for i in range(8)], asynchronous=True)
+        with torch.cuda.stream(side):
+            state, history = (x.clone() for x in pool.view(7))
+        side.synchronize()
+        m, h = pool.read(7)
+    finally:
+        backend.set_stream(None)
+    assert np.array_equal(state.cpu().numpy(), m) and np.array_equal(history.cpu().numpy(), h)
+    assert not np.array_equal(m, held[7][0])
+    pool.destroy()
+
+
+def test_view_without_history(backend):
+    pool = pkg.GdnState(backend, 1, 1, 32, 16, 1, 1)
+    m = np.arange(16 * 32, dtype=np.float32).reshape(1, 16, 32)
+    pool.write(pool.open(), m, np.zeros((pool.channels, 0), np.float32))
+    state, history = pool.view(0)
+    assert np.array_equal(state.cpu().numpy(), m) and history.shape == (pool.channels, 0)
+    pool.destroy()
