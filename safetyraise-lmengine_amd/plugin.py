@@ -776,7 +776,8 @@ class GdnState:
         import torch
 
         if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("gdn_view cannot be captured into a graph")
+            raise PluginError(STATUS_INVALID_ARGUMENT, "gdn_view",
+                              "gdn_view cannot be captured into a HIP graph")
         matrix, history = C.c_void_p(), C.c_void_p()
         self._call("view", seq, C.byref(matrix), C.byref(history))
         first = torch.cuda.current_device()

@@ -160,6 +160,6 @@ def test_another_device_is_current(library, home, current):
 
 def test_no_view_under_capture(library):
     library.capturing = True
-    with pytest.raises(RuntimeError, match="captured"):
+    with pytest.raises(pkg.PluginError, match="cannot be captured"):
         new_pool(library).view(0)
     assert "view" not in library.log
