@@ -339,6 +339,31 @@ def _is_device(x) -> bool:
     return x is not None and not isinstance(x, np.ndarray) and getattr(x, "is_cuda", False)
 
 
+_FLOAT = ("float32",)
+_ACTS = ("float32", "bfloat16")
+
+
+def _check_buffers(like, rows) -> None:
+    """Types, sizes and places of a call's buffers, which the library cannot see: rows
+    of (name, buffer, values, types); all of them are where `like` is.  Addresses
+    are taken as they are."""
+    for name, x, values, types in rows:
+        if x is None or isinstance(x, int):
+            continue
+        kind = str(x.dtype).replace("torch.", "")
+        if kind not in types:
+            raise TypeError(f"{name} is {kind}, not {' or '.join(types)}")
+        count = x.size if isinstance(x, np.ndarray) else x.numel()
+        if count < values:
+            raise ValueError(f"{name} has {count} values, the call {values}")
+        if not isinstance(like, int) and _is_device(x) != _is_device(like):
+            raise ValueError(f"{name} is not where the call's other buffers are")
+
+
+def _type_of(x):
+    return _ACTS if x is None or isinstance(x, int) else (str(x.dtype).replace("torch.", ""),)
+
+
 class NativeBackend:
     """Loaded plugin with one resident context (src/backend/mod.rs:137-234)."""
 
@@ -562,7 +587,9 @@ def attention_forward(backend: NativeBackend, kv: KvCache, seq_ids: Sequence[int
                       eps: float = 1e-6, q_norm=None, k_norm=None, gated: bool = False,
                       norm_offset: bool = False, mrope_section=(0, 0, 0),
                       mrope_interleaved: bool = True, asynchronous: bool = False) -> None:
-    """Attention::forward row loop (src/model/native.rs:615-645) for a batch."""
+    """Attention::forward row loop (src/model/native.rs:615-645) for a batch.  out is
+    float32."""
+    _check_buffers(out, [("out", out, 0, _FLOAT)])
     args = _attention_args(kv, seq_ids, seq_rows, q, k, v, positions, out, heads, kv_heads, head_dim,
                            rotary_dim, rope_theta, eps, q_norm, k_norm, gated, norm_offset,
                            mrope_section, mrope_interleaved, asynchronous)
@@ -625,6 +652,14 @@ def attention_tree_forward(backend: NativeBackend, kv: KvCache, seq_ids: Sequenc
     """attention_forward for trees of drafts: row r sees the context, its ancestors
     (parents[r]: a row of the same sequence, -1 behind the context) and itself.
     out is float32, or bfloat16 (a torch tensor)."""
+    # (a sequence of too many rows is the library's to refuse)
+    n = sum(seq_rows) if all(r <= MAX_TREE_ROWS for r in seq_rows) else 0
+    acts = _type_of(q)
+    _check_buffers(q, [
+        ("q", q, n * heads * head_dim * (2 if gated else 1), _ACTS),
+        ("k", k, n * kv_heads * head_dim, acts), ("v", v, n * kv_heads * head_dim, acts),
+        ("positions", positions, 3 * n, ("int32",)), ("q_norm", q_norm, head_dim, _FLOAT),
+        ("k_norm", k_norm, head_dim, _FLOAT), ("out", out, n * heads * head_dim, _ACTS)])
     args = AttentionTreeArgs()
     args.struct_size = C.sizeof(AttentionTreeArgs)
     args.attention = _attention_args(kv, seq_ids, seq_rows, q, k, v, positions, out, heads, kv_heads,
@@ -665,6 +700,8 @@ def kv_gather(backend: NativeBackend, reads, keys, values, asynchronous: bool = 
         else:
             lists.append((C.c_uint32 * max(1, len(tokens)))(*tokens))
             e.count, e.tokens = len(tokens), lists[-1]
+    total = sum(e.count for e in entries) * (reads[0][0].width if reads else 0)
+    _check_buffers(keys, [("keys", keys, total, _ACTS), ("values", values, total, _type_of(keys))])
     flags = 0
     if _is_device(keys):
         flags |= DEVICE_POINTERS | (ASYNC if asynchronous else 0)
@@ -811,7 +848,9 @@ def gdn_forward(backend: NativeBackend, state: GdnState, seq_ids: Sequence[int],
                 seq_rows: Sequence[int], qkv, z, a, b, a_log, dt_bias, conv_weight, norm, out,
                 *, eps: float = 1e-6, asynchronous: bool = False, keep_rows: bool = False) -> None:
     """Gdn::forward row loop (src/model/native.rs:720-742) for a batch; keep_rows
-    records every row so that GdnState.rollback can return to any of them."""
+    records every row so that GdnState.rollback can return to any of them.  out is
+    float32."""
+    _check_buffers(out, [("out", out, 0, _FLOAT)])
     args = _gdn_args(state, seq_ids, seq_rows, qkv, z, a, b, a_log, dt_bias, conv_weight, norm, out,
                      eps, asynchronous)
     args.flags |= KEEP_ROWS if keep_rows else 0
@@ -850,6 +889,15 @@ def gdn_tree_forward(backend: NativeBackend, state: GdnState, seq_ids: Sequence[
                      asynchronous: bool = False) -> None:
     """gdn_forward for trees of drafts (parents as in attention_tree_forward): each
     row continues from its parent; the states stay until gdn_tree_commit."""
+    n = sum(seq_rows) if all(r <= MAX_GDN_TREE_ROWS for r in seq_rows) else 0
+    width = state.value_heads * state.value_dim
+    acts = _type_of(qkv)
+    _check_buffers(qkv, [
+        ("qkv", qkv, n * state.channels, _ACTS), ("z", z, n * width, acts),
+        ("a", a, n * state.value_heads, acts), ("b", b, n * state.value_heads, acts),
+        ("a_log", a_log, state.value_heads, _FLOAT), ("dt_bias", dt_bias, state.value_heads, _FLOAT),
+        ("conv_weight", conv_weight, state.channels * state.conv_kernel, _FLOAT),
+        ("norm", norm, state.value_dim, _FLOAT), ("out", out, n * width, _FLOAT)])
     args = GdnTreeArgs()
     args.struct_size = C.sizeof(GdnTreeArgs)
     args.gdn = _gdn_args(state, seq_ids, seq_rows, qkv, z, a, b, a_log, dt_bias, conv_weight, norm,
