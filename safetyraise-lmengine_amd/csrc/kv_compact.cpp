@@ -312,7 +312,7 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
         move->start = (uint32_t)e.start;
         move->first_page = (uint32_t)p.first;
         move->pages = (uint32_t)(list - w.at);
-        std::memcpy(list, now.data(), now.size() * 4);
+        if (!now.empty()) std::memcpy(list, now.data(), now.size() * 4);
         list += now.size();
         if (!p.ranges.empty() && e.count > 0) {
             Lists::One &l = lists.lists[list_of[i]];

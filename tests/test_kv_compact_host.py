@@ -225,3 +225,16 @@ def test_gather_shares_a_list(host):  # noqa: F811
     assert status == 0
     want = [x.held[s][0][[start + t for t in tokens]] for x, s, start in ((m, a, 0), (other, b, 200), (m, a, 49))]
     assert np.array_equal(k, np.concatenate(want)) and np.array_equal(v, -k)
+
+
+def test_no_copies_from_nowhere(host):  # noqa: F811
+    """Entries without pages or tokens copy nothing (a copy of no bytes may not name no
+    address either)."""
+    m = Model(host)
+    a, b, c = m.new(40), m.new(20), m.new(0)
+    before = host.test.test_null_copies()
+    assert call(host, [(m, a, a, 0, []), (m, b, c, 0, []), ]) == 0
+    m.check()
+    assert call(host, [(m, c, c, 0, []), (m, b, b, 20, [])]) == 0
+    m.check()
+    assert host.test.test_null_copies() == before
