@@ -153,6 +153,22 @@ uint64_t next_call() {
     return ++calls;
 }
 
+// Shared pages of the pool that no sequence holds but targets of the call, which give
+// them up before any entry takes one.  (Pages of one target alone are counted for
+// every call; this walk over the pool is for one that would be short of pages.)
+uint64_t given_up_together(const safetyraise_kernel_kv_keep *entries, uint32_t n, const Pool *pool) {
+    std::vector<uint32_t> targets(pool->num_pages);
+    uint64_t pages = 0;
+    for (uint32_t i = 0; i < n; ++i) {
+        const auto &e = entries[i];
+        if (e.kv != pool || e.target == e.source) continue;
+        for (int32_t page : pool->seqs[e.target].pages) {
+            if (pool->refcount[page] > 1 && ++targets[page] == pool->refcount[page]) ++pages;
+        }
+    }
+    return pages;
+}
+
 int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n, uint32_t flags) {
     if (entries == nullptr || n == 0 || (flags & ~SAFETYRAISE_MI355X_ASYNC) != 0) {
         return fail(ctx, kInvalid, "kv_compact needs entries, and no flag but ASYNC");
@@ -195,7 +211,7 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
         if (st != kOk) return st;
     }
 
-    // plans, against the pages that are free now or that a target gives up
+    // plans, against the pages that are free now or that targets give up
     std::vector<KnownPlan> known;
     std::vector<uint32_t> plan_of(n);
     size_t ranges = 0, links = 0, words = 0;
@@ -227,6 +243,10 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
         }
         const CompactPlan &p = known[at].plan;
         plan_of[i] = (uint32_t)at;
+        if (p.fresh > pool->compact_free && pool->compact_shared != id) {
+            pool->compact_shared = id;
+            pool->compact_free += given_up_together(entries, n, pool);
+        }
         if (p.fresh > pool->compact_free) return fail(ctx, kNoMemory, "KV page pool exhausted");
         pool->compact_free -= p.fresh;
         ranges += p.ranges.size();

@@ -176,6 +176,7 @@ struct safetyraise_kernel_kv_pool {
     };
     std::vector<Sequence> seqs;
     uint64_t compact_call = 0, compact_free = 0;  // free pages left to a kv_compact call's entries
+    uint64_t compact_shared = 0;                  // the call whose targets' shared pages are among them
     std::vector<uint32_t> refcount;
     std::vector<int32_t> free_pages;
     size_t page_elems() const { return (size_t)kv_heads * page_tokens * head_dim; }

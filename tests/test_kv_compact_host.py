@@ -238,3 +238,38 @@ def test_no_copies_from_nowhere(host):  # noqa: F811
     assert call(host, [(m, c, c, 0, []), (m, b, b, 20, [])]) == 0
     m.check()
     assert host.test.test_null_copies() == before
+
+
+def test_pages_that_only_targets_share(host):  # noqa: F811
+    """Targets of one call that share pages with each other alone give them up together:
+    they count as free pages."""
+    m = Model(host, pages=20)
+    parent = m.new(128)  # 8 pages
+    a, b = m.fork(parent), m.fork(parent)
+    m.close(parent)
+    source, other = m.new(90), m.new(90)  # 6 pages each: the pool is full
+    assert m.free == 0
+    scattered = list(range(0, 90, 2))  # 3 pages of their own
+    assert call(host, [(m, source, a, 0, scattered), (m, other, b, 0, scattered)]) == 0
+    m.check()
+    m.pool.destroy()
+
+
+def test_pages_that_others_share_too(host):  # noqa: F811
+    """... but not where another sequence, or the entry's own source, holds them."""
+    m = Model(host, pages=20)
+    parent = m.new(128)
+    a, b = m.fork(parent), m.fork(parent)
+    source = m.new(190)  # 12 pages
+    assert m.free == 0
+    scattered = list(range(0, 128, 2))
+    assert call(host, [(m, source, a, 0, scattered), (m, source, b, 0, scattered)]) == 4
+    m.check()
+    assert call(host, [(m, parent, a, 0, scattered), (m, source, b, 0, scattered)]) == 4
+    m.check()
+    m.close(parent)
+    assert call(host, [(m, a, b, 0, scattered)]) == 4  # (a keeps the pages)
+    m.check()
+    assert call(host, [(m, source, a, 0, scattered), (m, source, b, 0, scattered)]) == 0
+    m.check()
+    m.pool.destroy()
