@@ -266,7 +266,15 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
     int32_t st = w.open(ctx, words, kMoveInlineWords);
     if (st != kOk) return st;
 
+    // what the targets were, so that a call whose launch fails leaves them so
+    struct Before {
+        std::vector<int32_t> pages;  // of another sequence than the source
+        uint64_t len;
+        size_t given_up;             // in place: pages of the list below
+    };
+    std::vector<Before> before(n);
     std::vector<MoveLink> late;
+    std::vector<uint32_t> late_of;
     std::vector<std::pair<Pool *, int32_t>> given_up;
     std::vector<int32_t> now;
     size_t most = 0, old_pages = 0;
@@ -275,10 +283,13 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
         const CompactPlan &p = known[plan_of[i]].plan;
         auto &target = e.kv->seqs[e.target];
         most = std::max(most, p.take.size());
-        if (e.target == e.source) old_pages += target.pages.size() - p.first;
-        target.pages.reserve(p.first + p.take.size());
+        before[i].len = target.len;
+        before[i].given_up = e.target == e.source ? target.pages.size() - p.first : 0;
+        old_pages += before[i].given_up;
+        (e.target == e.source ? target.pages : before[i].pages).reserve(p.first + p.take.size());
     }
     late.reserve(n);
+    late_of.reserve(n);
     given_up.reserve(old_pages);
     now.reserve(most);
 
@@ -291,8 +302,38 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
         for (int32_t page : t.pages) {
             if (--e.kv->refcount[page] == 0) e.kv->free_pages.push_back(page);
         }
-        t.pages.clear();
+        t.pages.swap(before[i].pages);
     }
+    // all of it taken back, the last step first
+    auto undo = [&]() {
+        auto hold = [](Pool *pool, int32_t page) {
+            if (pool->refcount[page]++ == 0) pool->free_pages.pop_back();
+        };
+        for (size_t k = given_up.size(); k-- > 0;) hold(given_up[k].first, given_up[k].second);
+        for (uint32_t i = n; i-- > 0;) {
+            const auto &e = entries[i];
+            const CompactPlan &p = known[plan_of[i]].plan;
+            auto &t = e.kv->seqs[e.target];
+            for (size_t q = p.take.size(); q-- > 0;) {
+                const int32_t page = t.pages[p.first + q];
+                if (--e.kv->refcount[page] == 0) e.kv->free_pages.push_back(page);
+            }
+            t.len = before[i].len;
+            if (e.target != e.source) {
+                t.pages.swap(before[i].pages);
+                continue;
+            }
+            t.pages.resize(p.first);
+            for (size_t k = given_up.size() - before[i].given_up; k < given_up.size(); ++k) t.pages.push_back(given_up[k].second);
+            given_up.resize(given_up.size() - before[i].given_up);
+        }
+        for (uint32_t i = n; i-- > 0;) {
+            const auto &e = entries[i];
+            if (e.target == e.source) continue;
+            const auto &pages = e.kv->seqs[e.target].pages;
+            for (size_t q = pages.size(); q-- > 0;) hold(e.kv, pages[q]);
+        }
+    };
     MoveEntry *move = (MoveEntry *)w.at;
     MoveRange *head = (MoveRange *)(move + n), *tail = head + chains;
     MoveRange *const first_range = head;
@@ -346,7 +387,7 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
         if (changed && !now.empty()) {
             const MoveLink l{pool->d_page_table + (size_t)e.target * pool->pages_per_seq + p.first,
                              move->pages, (uint32_t)now.size()};
-            if (in_place) late.push_back(l);
+            if (in_place) late.push_back(l), late_of.push_back(i);
             else *link++ = l, ++call.links;
         }
         MoveRange *last = nullptr;
@@ -380,8 +421,31 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
     call.words = (uint32_t)(list - w.at);
     if (call.chains + call.links + call.late_links > 0) {
         st = w.send(ctx, call.words, &call.device_words);
-        if (st != kOk) return st;
-        SR_HIP(ctx, launch_kv_moves(ctx->stream, call));
+        if (st == kOk) {
+            const hipError_t e = launch_kv_moves(ctx->stream, call);
+            if (e != hipSuccess) st = hip_fail(ctx, e, "kv_compact launch");
+        }
+        if (st != kOk) {
+            undo();
+            return st;
+        }
+        const hipError_t e = launch_kv_links(ctx->stream, call);
+        if (e != hipSuccess) {
+            // the tokens have moved: the rows of the page tables follow by another launch
+            st = hip_fail(ctx, e, "kv_compact page tables");
+            const std::string saved = ctx->error;
+            for (uint32_t i : late_of) {
+                Pool *pool = entries[i].kv;
+                TableBatch batch;
+                for (size_t q = known[plan_of[i]].plan.first; q < pool->seqs[entries[i].target].pages.size(); ++q) {
+                    batch.idx.push_back((uint32_t)(entries[i].target * pool->pages_per_seq + q));
+                    batch.val.push_back(pool->seqs[entries[i].target].pages[q]);
+                }
+                (void)kv_flush_table(ctx, pool, batch);
+            }
+            ctx->error = saved;
+            return st;
+        }
     }
     return finish_call(ctx, async);
 }

@@ -191,8 +191,9 @@ __global__ void __launch_bounds__(256) kv_gather_rows_kernel(const GatherArgs a)
 
 }  // namespace
 
-hipError_t launch_kv_moves(hipStream_t stream, const MoveCall &c) {
-    MoveArgs a{};
+namespace {
+
+bool move_args(const MoveCall &c, MoveArgs &a) {
     a.words = c.device_words;
     a.entries = c.entries;
     a.ranges = c.ranges;
@@ -200,19 +201,28 @@ hipError_t launch_kv_moves(hipStream_t stream, const MoveCall &c) {
     a.links = c.links;
     a.log2_heads = c.log2_heads;
     if (a.words == nullptr) {
-        if (c.words > kMoveInlineWords) return hipErrorInvalidValue;
+        if (c.words > kMoveInlineWords) return false;
         for (uint32_t i = 0; i < c.words; ++i) a.inline_words[i] = c.host_words[i];
     }
-    if (c.chains + c.links > 0) {
-        SR_LAUNCH("kv_move_kernel", kv_move_kernel, dim3(c.chains + c.links, 2 * c.head_groups), dim3(256),
-                  0, stream, a);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-    }
-    if (c.late_links > 0) {
-        SR_LAUNCH("kv_link_kernel", kv_link_kernel, dim3(c.late_links), dim3(256), 0, stream,
-                  c.device_words, a);
-    }
+    return true;
+}
+
+}  // namespace
+
+hipError_t launch_kv_moves(hipStream_t stream, const MoveCall &c) {
+    if (c.chains + c.links == 0) return hipSuccess;
+    MoveArgs a{};
+    if (!move_args(c, a)) return hipErrorInvalidValue;
+    SR_LAUNCH("kv_move_kernel", kv_move_kernel, dim3(c.chains + c.links, 2 * c.head_groups), dim3(256),
+              0, stream, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_links(hipStream_t stream, const MoveCall &c) {
+    if (c.late_links == 0) return hipSuccess;
+    MoveArgs a{};
+    if (!move_args(c, a)) return hipErrorInvalidValue;
+    SR_LAUNCH("kv_link_kernel", kv_link_kernel, dim3(c.late_links), dim3(256), 0, stream, c.device_words, a);
     return hipGetLastError();
 }
 

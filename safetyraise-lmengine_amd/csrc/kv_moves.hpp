@@ -74,7 +74,9 @@ struct GatherCall {
     void *keys, *values;
     bool bf16_out;
 };
+// the moves, and the rows that no range reads; then the other rows
 hipError_t launch_kv_moves(hipStream_t stream, const MoveCall &call);
+hipError_t launch_kv_links(hipStream_t stream, const MoveCall &call);
 hipError_t launch_kv_gather_rows(hipStream_t stream, const GatherCall &call);
 
 }  // namespace sr

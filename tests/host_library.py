@@ -34,10 +34,10 @@ def host(host_path):
     backend = pkg.NativeBackend.load(host_path)
     test = backend.test = C.CDLL(str(host_path))
     test.test_seed.argtypes = [C.c_uint64]
-    test.test_fail.argtypes = [C.c_char_p]
+    test.test_fail.argtypes = [C.c_char_p, C.c_int]
     test.test_pool.argtypes = [C.c_void_p]
     test.test_free_pages.argtypes = [C.c_void_p]
     test.test_free_pages.restype = C.c_uint64
-    test.test_fail(b"")
+    test.test_fail(b"", 0)
     yield backend
     backend.close()

@@ -273,3 +273,60 @@ def test_pages_that_others_share_too(host):  # noqa: F811
     assert call(host, [(m, source, a, 0, scattered), (m, source, b, 0, scattered)]) == 0
     m.check()
     m.pool.destroy()
+
+
+def lists_of(m):
+    """Everything of a pool that a refused call may not change."""
+    return m.free, {s: m.pool.len(s) for s in m.held}
+
+
+@pytest.mark.parametrize("launch", ["linear_input", "kv_moves"])
+def test_a_launch_that_fails_changes_nothing(host, launch):  # noqa: F811
+    """Page lists, reference counts, free pages and tables are as before the call, and the
+    same call can be made again."""
+    rng = np.random.default_rng(5)
+    failed = 0
+    for turn in range(120):
+        models = [Model(host, 16, int(rng.integers(60, 130))) for _ in range(3)]
+        entries = []
+        for m in models:
+            a, b, c = (m.new(int(rng.integers(100, 300))) for _ in range(3))
+            if rng.random() < 0.6:
+                m.fork(int(rng.choice([a, b, c])))
+            lengths = [len(m.held[s][0]) for s in (a, b)]
+            kept = [sorted(rng.choice(n - 20, int(n * rng.choice([0.4, 0.95])) - 20, replace=False).tolist())
+                    for n in lengths]
+            entries += [(m, a, a, 20, kept[0]), (m, b, c, 20, kept[1])]
+        before = [lists_of(m) for m in models]
+        host.test.test_fail(launch.encode(), 0)
+        status = call(host, entries)
+        if host.test.test_failing():  # too few pages; or few enough tokens for the arguments
+            assert status in (0, 4)
+            host.test.test_fail(b"", 0)
+            continue
+        assert status == 5
+        failed += 1
+        assert [lists_of(m) for m in models] == before
+        for m in models:
+            m.check()
+        assert call(host, entries) == 0
+        for m in models:
+            m.check()
+            m.pool.destroy()
+    assert failed > 15
+
+
+def test_a_page_table_launch_that_fails(host):  # noqa: F811
+    """The tokens have moved in place by then: the call reports the error, and the
+    sequences are what it made them."""
+    m = Model(host, pages=160)
+    a, b = m.new(900), m.new(200)
+    kept = [t for t in range(880) if not 30 <= t < 130]
+    host.test.test_fail(b"kv_links", 0)
+    rows = m.kept(a, 20, kept), m.kept(b, 7, [100, 101, 190])
+    assert call(host, [(m, a, a, 20, kept), (m, b, b, 7, [100, 101, 190])]) == 5
+    assert not host.test.test_failing()
+    m.held[a], m.held[b] = rows
+    m.check()
+    m.append(a, 50)
+    m.check()
