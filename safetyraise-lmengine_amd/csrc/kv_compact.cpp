@@ -261,7 +261,13 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
     const size_t fixed = (n * sizeof(MoveEntry) + ranges * sizeof(MoveRange) + links * sizeof(MoveLink)) / 4;
     words += fixed;
     for (const Lists::One &l : lists.lists) words += l.count;
-    if (words > UINT32_MAX) return fail(ctx, kOverflow, "kv_compact is too large for one call");
+    // short ranges: a workgroup takes as many heads as it has in flight at once
+    uint32_t log2_heads = 0;
+    while ((2u << log2_heads) <= kv_heads && (longest << (log2_heads + 1)) <= in_flight) ++log2_heads;
+    const uint32_t head_groups = (kv_heads + (1u << log2_heads) - 1) >> log2_heads;
+    if (words > UINT32_MAX || (uint64_t)chains + links > kMostBlocks || head_groups > kMostBlocksY / 2) {
+        return fail(ctx, kOverflow, "kv_compact is too large for one call");
+    }
     Words w;
     int32_t st = w.open(ctx, words, kMoveInlineWords);
     if (st != kOk) return st;
@@ -414,9 +420,8 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
     call.chains = chains;
     call.ranges = (uint32_t)ranges;
     call.late_links = (uint32_t)late.size();
-    // short ranges: a workgroup takes as many heads as it has in flight at once
-    while ((2u << call.log2_heads) <= kv_heads && (longest << (call.log2_heads + 1)) <= in_flight) ++call.log2_heads;
-    call.head_groups = (kv_heads + (1u << call.log2_heads) - 1) >> call.log2_heads;
+    call.log2_heads = log2_heads;
+    call.head_groups = head_groups;
     call.host_words = w.at;
     call.words = (uint32_t)(list - w.at);
     if (call.chains + call.links + call.late_links > 0) {
@@ -509,7 +514,7 @@ int32_t gather(Ctx *ctx, const safetyraise_kernel_kv_rows *entries, uint32_t n, 
     }
     uint64_t words = (call.entries * sizeof(GatherEntry) + blocks * sizeof(GatherBlock)) / 4;
     for (const Lists::One &l : lists.lists) words += l.count;
-    if (words > UINT32_MAX || blocks > INT32_MAX) return fail(ctx, kOverflow, "kv_gather is too large for one call");
+    if (words > UINT32_MAX || blocks > kMostBlocks) return fail(ctx, kOverflow, "kv_gather is too large for one call");
     Words w;
     int32_t st = w.open(ctx, words, kGatherInlineWords);
     if (st != kOk) return st;

@@ -50,6 +50,9 @@ static_assert(sizeof(MoveEntry) % 8 == 0 && sizeof(MoveRange) % 8 == 0 && sizeof
 constexpr uint32_t kMoveInlineWords = 1008;  // what fits the kernel arguments
 constexpr uint32_t kGatherInlineWords = 992;
 
+// Workgroups of 256 threads that a launch has at most: its threads are counted in 32 bits.
+constexpr uint32_t kMostBlocks = UINT32_MAX / 256, kMostBlocksY = 65535;
+
 // Rows (one token of one head) that a workgroup of the move kernel has in flight.
 constexpr uint32_t kMovePasses = 4;
 constexpr uint32_t move_rows(uint32_t head_dim) {

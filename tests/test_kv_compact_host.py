@@ -330,3 +330,17 @@ def test_a_page_table_launch_that_fails(host):  # noqa: F811
     m.check()
     m.append(a, 50)
     m.check()
+
+
+def test_gather_past_a_launch(host):  # noqa: F811
+    """More workgroups than a launch has are refused."""
+    pool = pkg.KvCache(host, 1, 510, 16, 1, 16, 1)
+    s = pool.open()
+    rows = np.zeros((1, 510), np.float32)
+    pool.append(s, rows, rows)
+    reads = (pkg.plugin.KvRows * 1)()
+    count = 1 << 25  # two tokens to a workgroup
+    tokens = (C.c_uint32 * count)()
+    reads[0].kv, reads[0].sequence, reads[0].count, reads[0].tokens = pool.handle, s, count, tokens
+    assert host.lib.safetyraise_kernel_kv_gather(host.context, reads, 1, rows.ctypes.data, rows.ctypes.data, 0) == 3
+    pool.destroy()
