@@ -61,7 +61,8 @@ extern "C" {
 #define SAFETYRAISE_MI355X_GATED UINT32_C(0x20)      /* q rows are per-head [q, gate] */
 #define SAFETYRAISE_MI355X_MROPE_INTERLEAVED UINT32_C(0x40)
 #define SAFETYRAISE_MI355X_KEEP_ROWS UINT32_C(0x80) /* gdn_forward: allow gdn_rollback */
-#define SAFETYRAISE_MI355X_OUTPUT_BF16 UINT32_C(0x100) /* bf16 output (attention_tree_forward, kv_gather) */
+/* bf16 output (attention_tree_forward, kv_gather; the calls that write f32 refuse it) */
+#define SAFETYRAISE_MI355X_OUTPUT_BF16 UINT32_C(0x100)
 
 /* Largest number of sequences one call may carry. */
 #define SAFETYRAISE_MI355X_MAX_BATCH 1024u

@@ -221,6 +221,9 @@ int32_t attention_forward_impl(Ctx *ctx, const safetyraise_kernel_attention_args
     const bool qk_norm = (flags & SAFETYRAISE_MI355X_QK_NORM) != 0;
     if (pool == nullptr) return fail(ctx, kInvalid, "attention needs a KV pool");
     if (async && !device) return fail(ctx, kInvalid, "ASYNC needs DEVICE_POINTERS");
+    if ((flags & SAFETYRAISE_MI355X_OUTPUT_BF16) != 0) {
+        return fail(ctx, kInvalid, "attention_forward writes f32: it takes no OUTPUT_BF16");
+    }
     // causal_attention geometry (math.rs:109-124)
     if (A.heads == 0 || A.kv_heads == 0 || A.head_dim == 0 || A.heads % A.kv_heads != 0 ||
         A.kv_heads != pool->kv_heads || A.head_dim != pool->head_dim) {

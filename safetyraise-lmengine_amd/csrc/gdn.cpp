@@ -238,6 +238,9 @@ SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_forward(
     const bool bf16 = (A.flags & SAFETYRAISE_MI355X_INPUT_BF16) != 0;
     if (pool == nullptr) return fail(ctx, kInvalid, "gdn_forward needs a state pool");
     if (async && !device) return fail(ctx, kInvalid, "ASYNC needs DEVICE_POINTERS");
+    if ((A.flags & SAFETYRAISE_MI355X_OUTPUT_BF16) != 0) {
+        return fail(ctx, kInvalid, "gdn_forward writes f32: it takes no OUTPUT_BF16");
+    }
     if (!std::isfinite(A.eps) || A.eps <= 0.0f) {
         return fail(ctx, kInvalid, "RMSNorm shape or epsilon is invalid");
     }

@@ -42,6 +42,9 @@ int32_t tree_forward(Ctx *ctx, const safetyraise_kernel_gdn_tree_args *args) {
     const bool bf16 = (A.flags & SAFETYRAISE_MI355X_INPUT_BF16) != 0;
     if (pool == nullptr) return fail(ctx, kInvalid, "gdn_tree_forward needs a state pool");
     if (async && !device) return fail(ctx, kInvalid, "ASYNC needs DEVICE_POINTERS");
+    if ((A.flags & SAFETYRAISE_MI355X_OUTPUT_BF16) != 0) {
+        return fail(ctx, kInvalid, "gdn_tree_forward writes f32: it takes no OUTPUT_BF16");
+    }
     if ((A.flags & SAFETYRAISE_MI355X_KEEP_ROWS) != 0) {
         return fail(ctx, kInvalid, "gdn_tree_forward takes no KEEP_ROWS: it records every row");
     }
