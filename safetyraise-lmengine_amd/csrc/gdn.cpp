@@ -360,13 +360,17 @@ SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_forward(
     g.records = pool->d_records;
     g.rec_stride = (uint32_t)pool->record_elems();
     g.keep_rows = pool->keep_rows;
+    // from the first launch on, the records and the other buffers are no earlier call's
+    for (const GdnSeq &q : seqs) {
+        pool->kept[q.slot] = Pool::kNoKept;
+        pool->trees[q.slot].parents.clear();
+    }
     SR_HIP(ctx, launch_gdn(ctx->stream, g, seqs.data(), (int)A.num_seqs, (uint32_t)total));
     for (const GdnSeq &q : seqs) {
         pool->parity[q.slot] ^= 1u;
         if (keep) pool->state_par[q.slot] ^= 1u;
         pool->kept[q.slot] = keep ? q.rows : Pool::kNoKept;
         pool->kept_at[q.slot] = q.rows;
-        pool->trees[q.slot].parents.clear();
     }
     if (!device) {
         SR_HIP(ctx, hipMemcpyAsync(A.out, g.out, out_b, hipMemcpyDeviceToHost, ctx->stream));

@@ -156,6 +156,11 @@ int32_t tree_forward(Ctx *ctx, const safetyraise_kernel_gdn_tree_args *args) {
     for (uint32_t i = 0; i < A.num_seqs; ++i) {
         kept[i].assign(args->parents + seqs[i].row0, args->parents + seqs[i].row0 + seqs[i].rows);
     }
+    // from the first launch on, the records are no earlier call's
+    for (const GdnSeq &q : seqs) {
+        pool->kept[q.slot] = Pool::kNoKept;
+        pool->trees[q.slot].parents.clear();
+    }
     for (uint32_t i = 0; i < A.num_seqs; i += kGdnTreeSeqs) {
         const int n = (int)std::min<uint32_t>(kGdnTreeSeqs, A.num_seqs - i);
         SR_HIP(ctx, launch_gdn_tree(ctx->stream, g, &seqs[i], n, parents.data() + seqs[i].row0,
@@ -167,7 +172,6 @@ int32_t tree_forward(Ctx *ctx, const safetyraise_kernel_gdn_tree_args *args) {
         t.parents = std::move(kept[i]);
         t.state_par = pool->state_par[id];
         t.parity = pool->parity[id];
-        pool->kept[id] = Pool::kNoKept;
     }
     if (!device) {
         SR_HIP(ctx, hipMemcpyAsync(A.out, g.out, out_b, hipMemcpyDeviceToHost, ctx->stream));

@@ -1,6 +1,6 @@
 // The library's host code without a GPU: the runtime's calls on host memory, and the page
 // copies, table writes and token moves done there, the workgroups of a launch in random
-// order.  Calls that compute launch nothing and say so.  test_fail makes a launch fail.
+// order.  Calls that compute do nothing.  test_fail makes a launch fail.
 #include <cmath>
 #include <cstdlib>
 #include <cstring>
@@ -308,15 +308,16 @@ TreeScratch tree_scratch(const TreeLaunch &, const SeqMeta *, int, uint64_t, int
 hipError_t launch_tree_attn(hipStream_t, const TreeLaunch &, const SeqMeta *, int, const uint8_t *, const TreePlan &) {
     return hipErrorNotSupported;
 }
-hipError_t launch_gdn(hipStream_t, const GdnLaunch &, const GdnSeq *, int, uint32_t) { return hipErrorNotSupported; }
+// (launched, and computing nothing)
+hipError_t launch_gdn(hipStream_t, const GdnLaunch &, const GdnSeq *, int, uint32_t) { return launch("gdn"); }
 size_t gdn_chunk_rec_bytes(const safetyraise_kernel_gdn_pool *, const GdnSeq *, int, bool, bool) { return 0; }
-hipError_t launch_gdn_rollback(hipStream_t, const GdnRollback &) { return hipErrorNotSupported; }
+hipError_t launch_gdn_rollback(hipStream_t, const GdnRollback &) { return launch("gdn_rollback"); }
 size_t gdn_tree_scratch_bytes(const safetyraise_kernel_gdn_pool *, uint32_t) { return 0; }
 hipError_t launch_gdn_tree(hipStream_t, const GdnLaunch &, const GdnSeq *, int, const uint8_t *, float *) {
-    return hipErrorNotSupported;
+    return launch("gdn_tree");
 }
 hipError_t launch_gdn_tree_commit(hipStream_t, const GdnCommitEntry *, uint32_t, const GdnCommitEntry *) {
-    return hipErrorNotSupported;
+    return launch("gdn_tree_commit");
 }
 uint32_t gdn_key_dim() { return 128; }
 uint32_t gdn_row_block() { return 64; }
