@@ -27,6 +27,11 @@ namespace {
 
 constexpr uint32_t kRowsMax = kMaxGdnTreeRows;
 
+// Least log a that sums of them take: e^x is 0 in f32 from -104 on, and differences of
+// sums that hold minus infinity would be NaN.
+constexpr float kLeastLog = -1000.0f;
+__device__ __forceinline__ float finite_log(float log_a) { return log_a < kLeastLog ? kLeastLog : log_a; }
+
 struct TreeMeta {
     uint32_t slot, rows, row0, parity, state_in;
 };
@@ -115,7 +120,7 @@ __global__ void __launch_bounds__(256) gdn_tree_generic_kernel(const GdnTreePara
     if (tid < R) {
         const float av = load_act(p.a, (size_t)(m.row0 + tid) * p.value_heads + h, p.bf16_in);
         const float bv = load_act(p.b, (size_t)(m.row0 + tid) * p.value_heads + h, p.bf16_in);
-        log_a[tid] = -expf(p.a_log[h]) * softplus_ref(av + p.dt_bias[h]);
+        log_a[tid] = finite_log(-expf(p.a_log[h]) * softplus_ref(av + p.dt_bias[h]));
         beta[tid] = ref_sigmoid(bv);
         rec[(size_t)tid * p.rec_stride + h] = expf(log_a[tid]);
     }
@@ -402,7 +407,7 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
         asm volatile("" : "+v"(a_raw), "+v"(b_raw), "+v"(up_raw), "+v"(a_log), "+v"(dt_bias));
         const float av = __uint_as_float(bf16 ? a_raw << 16 : a_raw), bv = __uint_as_float(bf16 ? b_raw << 16 : b_raw);
         const int up = (int)up_raw - 1;
-        const float log_a = -expf(a_log) * softplus_ref(av + dt_bias);
+        const float log_a = finite_log(-expf(a_log) * softplus_ref(av + dt_bias));
         // the path's set and sum up to, not with, `next`: doubling
         int next = up;
         uint32_t lo = r < 32 ? 1u << r : 0u, hi = r < 32 ? 0u : 1u << (r - 32);
