@@ -315,6 +315,7 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
     __shared__ double g_s[kRowsMax];
     __shared__ uint64_t anc_s[kRowsMax];
     __shared__ float beta_s[kRowsMax], decay_s[kRowsMax];
+    __shared__ uint32_t lost_s[2];  // rows whose decay, step or key is not finite
     // a row's conv taps, newest first: byte offsets of their LDS rows
     __shared__ __align__(16) uint16_t tap_s[kRowsMax][8];
     float *xq = lds + 2 * T::kPart, *xk = lds, *xv = lds + 3 * T::kPart;
@@ -407,7 +408,12 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
         asm volatile("" : "+v"(a_raw), "+v"(b_raw), "+v"(up_raw), "+v"(a_log), "+v"(dt_bias));
         const float av = __uint_as_float(bf16 ? a_raw << 16 : a_raw), bv = __uint_as_float(bf16 ? b_raw << 16 : b_raw);
         const int up = (int)up_raw - 1;
-        const float log_a = finite_log(-expf(a_log) * softplus_ref(av + dt_bias));
+        const float raw_log = finite_log(-expf(a_log) * softplus_ref(av + dt_bias)), raw_beta = ref_sigmoid(bv);
+        // (rows that are not finite: see step 6)
+        const bool lost = isnan(raw_log) || isnan(raw_beta);
+        const uint64_t all_lost = __builtin_amdgcn_ballot_w64(lost && lane < R);
+        if (lane < 2) lost_s[lane] = (uint32_t)(all_lost >> (32 * lane));
+        const float log_a = lost ? 0.0f : raw_log, beta = lost ? 0.0f : raw_beta;
         // the path's set and sum up to, not with, `next`: doubling
         int next = up;
         uint32_t lo = r < 32 ? 1u << r : 0u, hi = r < 32 ? 0u : 1u << (r - 32);
@@ -440,9 +446,9 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
         if (lane < R) {
             g_s[lane] = sum;
             anc_s[lane] = ((uint64_t)hi << 32) | lo;
-            beta_s[lane] = ref_sigmoid(bv);
+            beta_s[lane] = beta;
             decay_s[lane] = (float)exp(sum);
-            rec[(size_t)lane * p.rec_stride + h] = expf(log_a);
+            rec[(size_t)lane * p.rec_stride + h] = expf(raw_log);
         } else {
             // rows of the last tile past the tree
             g_s[lane] = 0.0;
@@ -540,15 +546,20 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
                 for (uint32_t i = 0; i < kBatch; ++i) {
                     const uint32_t t = t0 + 8 * i;
                     if (t >= 16 * rt) break;
-                    const float a = y[i].x * inv[i], b = y[i].y * inv[i];
+                    float a = y[i].x * inv[i], b = y[i].y * inv[i];
+                    if (turn == 2) {
+                        if (first_of_key && t < R) *(f32x2u *)(keys + (size_t)t * rec_stride) = f32x2u{a, b};
+                        // (a key that is not finite would reach every row: 0 in its place)
+                        if (!(inv[i] > 0.0f) && __builtin_amdgcn_ballot_w64(!isfinite(a) || !isfinite(b)) != 0) {
+                            a = b = 0.0f;
+                            if (lane == 0) atomicOr(&lost_s[t >> 5], 1u << (t & 31));
+                        }
+                    }
                     constexpr float kScale = (float)(1 << kSplitExp);
                     const f16x2 hi = {(_Float16)(a * kScale), (_Float16)(b * kScale)};
                     const f16x2 lo = {(_Float16)(a * kScale - (float)hi.x), (_Float16)(b * kScale - (float)hi.y)};
                     ((f16x2 *)(to + t * kPitch))[lane] = hi;
                     ((f16x2 *)(to + t * kPitch))[64 + lane] = lo;
-                    if (turn == 2 && first_of_key && t < R) {
-                        *(f32x2u *)(keys + (size_t)t * rec_stride) = f32x2u{a, b};
-                    }
                 }
             }
             __syncthreads();
@@ -656,7 +667,20 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
         }
     }
     __syncthreads();
-    // 6.
+    // 6.  A row of d that is not finite is 0 in the products, or it would reach rows that
+    // do not see it (0 x inf); bits of such rows are kept per column.
+    uint64_t lost = 0;
+    auto finite_rows = [&](f32x4 x, int b) __attribute__((always_inline)) {
+        const float zero = fmaf(x[0], 0.0f, x[1] * 0.0f) + fmaf(x[2], 0.0f, x[3] * 0.0f);
+        if (__builtin_amdgcn_ballot_w64(zero != 0.0f) == 0) return x;  // (NaN is not 0)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const bool fine = isfinite(x[e]);
+            lost |= fine ? 0ull : 1ull << (16 * b + 4 * g4 + e);
+            x[e] = fine ? x[e] : 0.0f;
+        }
+        return x;
+    };
     const float qscale = 0.08838834764831845f;  // 1 / sqrt(128)
     f32x4 D[RT];
 #pragma unroll
@@ -677,13 +701,27 @@ __global__ void __launch_bounds__(512) gdn_tree_head_kernel(const GdnTreeParams 
             rhs = mma16(*(const f32x4 *)(Ar + 16 * cc), D[cc], rhs);
             o = mma16(*(const f32x4 *)(Pr + 16 * cc), D[cc], o);
         }
-        D[b] = mma16(*(const f32x4 *)(Ar + 16 * b), rhs, f32x4{});
+        D[b] = finite_rows(mma16(*(const f32x4 *)(Ar + 16 * b), finite_rows(rhs, b), f32x4{}), b);
         o = mma16(*(const f32x4 *)(Pr + 16 * b), D[b], o);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const uint32_t t = 16 * b + 4 * g4 + e;
             vr[e * kPitch] = o[e] * qscale;
             if (t < R) rec[(size_t)t * p.rec_stride + rec_delta(p) + h * kW + 16 * wave + l16] = D[b][e];
+        }
+    }
+    const uint64_t lost_rows = ((uint64_t)lost_s[1] << 32) | lost_s[0];
+    if (__builtin_amdgcn_ballot_w64((lost | lost_rows) != 0) != 0) {
+        // the rows that descend from such rows, in the columns where they are
+        uint32_t lo = (uint32_t)(lost | lost_rows), hi = (uint32_t)((lost | lost_rows) >> 32);
+        lo |= __shfl_xor(lo, 16), hi |= __shfl_xor(hi, 16);
+        lo |= __shfl_xor(lo, 32), hi |= __shfl_xor(hi, 32);
+        const uint64_t above = ((uint64_t)hi << 32) | lo;
+#pragma unroll 1
+        for (uint32_t t = g4; t < R; t += 4) {
+            if ((anc_s[t] & above) == 0) continue;
+            xv[t * kPitch + 16 * wave + l16] = NAN;
+            rec[(size_t)t * p.rec_stride + rec_delta(p) + h * kW + 16 * wave + l16] = NAN;
         }
     }
     __syncthreads();
