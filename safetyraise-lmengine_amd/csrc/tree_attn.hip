@@ -249,13 +249,25 @@ __global__ void __launch_bounds__(256) tree_prep_kernel(const PrepParams p) {
         if (hh < c.kv_heads) {
             const size_t base =
                 ((((size_t)hh * c.num_pages + page) << c.log2_page) + (tok & ((1u << c.log2_page) - 1))) * D;
+            // A value that is not finite would reach rows that do not see it (0 x inf in the
+            // products): such a row gets a key of NaN, which its own descendants'
+            // scores take up and the others' masks drop, and a value of 0.
+            uint16_t kb[NI], vb[NI];
+            bool fine = true;
+#pragma unroll
+            for (uint32_t i = 0; i < NI; ++i) {
+                kb[i] = f32_to_bf16(y[min(lane + 64 * i, D - 1)]);
+                vb[i] = f32_to_bf16(v[u][i]);
+                fine = fine && isfinite(bf16_to_f32(kb[i])) && isfinite(bf16_to_f32(vb[i]));
+            }
+            const bool lost = __builtin_amdgcn_ballot_w64(!fine) != 0;
+            finite = finite && !lost;
 #pragma unroll
             for (uint32_t i = 0; i < NI; ++i) {
                 const uint32_t d = lane + 64 * i;
                 if (d >= D) continue;
-                finite = finite && isfinite(y[d]) && isfinite(v[u][i]);
-                c.k_pages[base + d] = f32_to_bf16(y[d]);
-                c.v_pages[base + d] = f32_to_bf16(v[u][i]);
+                c.k_pages[base + d] = lost ? (uint16_t)0x7fc0u : kb[i];
+                c.v_pages[base + d] = lost ? (uint16_t)0u : vb[i];
             }
             continue;
         }
