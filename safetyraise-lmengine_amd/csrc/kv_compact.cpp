@@ -274,26 +274,26 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
 
     // what the targets were, so that a call whose launch fails leaves them so
     struct Before {
-        std::vector<int32_t> pages;  // of another sequence than the source
         uint64_t len;
-        size_t given_up;             // in place: pages of the list below
+        size_t pages;  // from the first changed one on, in one of the lists below
     };
     std::vector<Before> before(n);
+    std::vector<int32_t> replaced;  // of targets that are not their entry's source
     std::vector<MoveLink> late;
     std::vector<uint32_t> late_of;
     std::vector<std::pair<Pool *, int32_t>> given_up;
     std::vector<int32_t> now;
-    size_t most = 0, old_pages = 0;
+    size_t most = 0, old_pages = 0, others = 0;
     for (uint32_t i = 0; i < n; ++i) {
         const auto &e = entries[i];
         const CompactPlan &p = known[plan_of[i]].plan;
         auto &target = e.kv->seqs[e.target];
         most = std::max(most, p.take.size());
-        before[i].len = target.len;
-        before[i].given_up = e.target == e.source ? target.pages.size() - p.first : 0;
-        old_pages += before[i].given_up;
-        (e.target == e.source ? target.pages : before[i].pages).reserve(p.first + p.take.size());
+        before[i] = {target.len, target.pages.size() - p.first};
+        (e.target == e.source ? old_pages : others) += before[i].pages;
+        target.pages.reserve(p.first + p.take.size());
     }
+    replaced.reserve(others);
     late.reserve(n);
     late_of.reserve(n);
     given_up.reserve(old_pages);
@@ -308,7 +308,8 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
         for (int32_t page : t.pages) {
             if (--e.kv->refcount[page] == 0) e.kv->free_pages.push_back(page);
         }
-        t.pages.swap(before[i].pages);
+        replaced.insert(replaced.end(), t.pages.begin(), t.pages.end());
+        t.pages.clear();
     }
     // all of it taken back, the last step first
     auto undo = [&]() {
@@ -316,6 +317,7 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
             if (pool->refcount[page]++ == 0) pool->free_pages.pop_back();
         };
         for (size_t k = given_up.size(); k-- > 0;) hold(given_up[k].first, given_up[k].second);
+        size_t in_place = given_up.size(), other = replaced.size();
         for (uint32_t i = n; i-- > 0;) {
             const auto &e = entries[i];
             const CompactPlan &p = known[plan_of[i]].plan;
@@ -325,13 +327,14 @@ int32_t compact(Ctx *ctx, const safetyraise_kernel_kv_keep *entries, uint32_t n,
                 if (--e.kv->refcount[page] == 0) e.kv->free_pages.push_back(page);
             }
             t.len = before[i].len;
-            if (e.target != e.source) {
-                t.pages.swap(before[i].pages);
-                continue;
-            }
             t.pages.resize(p.first);
-            for (size_t k = given_up.size() - before[i].given_up; k < given_up.size(); ++k) t.pages.push_back(given_up[k].second);
-            given_up.resize(given_up.size() - before[i].given_up);
+            if (e.target == e.source) {
+                in_place -= before[i].pages;
+                for (size_t k = 0; k < before[i].pages; ++k) t.pages.push_back(given_up[in_place + k].second);
+            } else {
+                other -= before[i].pages;
+                t.pages.insert(t.pages.end(), replaced.begin() + other, replaced.begin() + other + before[i].pages);
+            }
         }
         for (uint32_t i = n; i-- > 0;) {
             const auto &e = entries[i];
