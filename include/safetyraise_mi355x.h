@@ -378,9 +378,13 @@ SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_forward(
  * accepted path with kv_compact.  At most MAX_TREE_ROWS rows per sequence.
  * out is f32, or bf16 with OUTPUT_BF16.  An f32 result carries f32 products
  * (q and the probabilities in three bf16 parts each, f32 sums); for a bf16
- * result q is used in two parts and the probabilities in one, roundings below
- * its own.  Any head_dim 1..512 and any group of query heads; 64, 128 and 256
- * take the MFMA kernel. */
+ * result the probabilities are used in one part, 2^-8 of each value that they
+ * weigh, as large as the result's own rounding, and q in two, 2^-16 of each
+ * product with a key: less than that while what a score sums in magnitude,
+ * sum |q k| / sqrt(head_dim), is below 2^8.  Any head_dim 1..512 and any
+ * group of query heads; 64, 128 and 256 take the MFMA kernel.
+ * A row whose key or value is not finite, as given or in bf16, is an error; of
+ * an asynchronous call's rows, those that do not descend from it are right. */
 typedef struct safetyraise_kernel_attention_tree_args {
     uint32_t struct_size;
     uint32_t reserved; /* 0 */

@@ -101,7 +101,11 @@ __global__ void __launch_bounds__(256) gdn_tree_conv_kernel(const GdnTreeParams 
     p.records[((size_t)m.slot * p.keep_rows + sr) * p.rec_stride + rec_raw(p) + c] = x;
 }
 
-// Any widths: one workgroup per (value head, sequence), a thread per value dim.
+// Any widths: one workgroup per (value head, sequence), a thread per value dim, which
+// goes through the rows one after another.  Bound by that chain and by the reads of its
+// state row for every row of the tree: eight sequences of 44 rows, 32 value heads of 64 x 64,
+// 340 us and 18 for the conv, where inputs, state and outputs are 3.3 us.  It is there for
+// widths that no configuration of this framework has.
 __global__ void __launch_bounds__(256) gdn_tree_generic_kernel(const GdnTreeParams p) {
     __shared__ float kk[kRowsMax][kRowsMax + 1], qk[kRowsMax][kRowsMax + 1];
     __shared__ double g[kRowsMax];
@@ -231,11 +235,11 @@ __global__ void __launch_bounds__(256) gdn_tree_generic_kernel(const GdnTreePara
 // RT: 16-row tiles of the longest tree.
 //
 // What bounds it: the chain of phases, each bound by something else.  Eight sequences of
-// 24..64 rows, 16 key and 32 value heads: 28.7 us for 40 MB (8.3 us at the copy rate):
+// 24..64 rows, 16 key and 32 value heads: 30.2 us for 40 MB (8.3 us at the copy rate):
 // inputs and state 7, conv and norms 6.3 (vector instructions: exponentials and
 // reciprocals of the silu; q and k are made once per value head of theirs), products 4.9,
-// solve 0.7, step 6 2.2, outputs 1.6.  One sequence of 12 rows: 10.6 us, mostly latency and
-// the fetch of the code.  With 4-byte loads, the conv in place and the norms in a pass
+// solve 0.7, step 6 2.2 and 0.8 more for its checks of d, outputs 1.6.  One sequence of 12
+// rows: 10.7 us, mostly latency and the fetch of the code.  With 4-byte loads, the conv in place and the norms in a pass
 // of their own it took 32 us.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kW = 128;         // Dk and Dv

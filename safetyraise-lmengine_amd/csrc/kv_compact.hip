@@ -3,8 +3,9 @@
 //
 // Both are copies: bound by the bytes they read and write, or for a few tokens by the
 // launch (4.6 us).  14500 of 53000 tokens of two sequences, 8 heads of width 128, to free
-// pages, 119 MB: 24 us; 33300 of three, 2 heads of width 256, to f32 rows, 205 MB: 37.5 us
-// where the last cache holds part of it, 43 where not.
+// pages, 119 MB: 29.4 us; 33300 of three, 2 heads of width 256, to f32 rows, 205 MB: 38.6 us
+// (each call with inputs of its own).  Serial ranges are bound by one workgroup's round
+// trips: 12800 tokens of two sequences in place, 105 MB, 29 us to free pages, 224 without any.
 //
 // The call's description (entries, ranges, token lists, page ids) travels in the
 // kernel arguments where it fits, else through pinned host memory into a device buffer.

@@ -327,7 +327,11 @@ __device__ __forceinline__ void store_out(const TreeCommon &c, size_t at, float 
 }
 
 // Any head width: one wave per (row, query head) over the visible keys in tiles
-// of 64, a key per lane for the scores and a dim per lane for the sums.
+// of 64, a key per lane for the scores and a dim per lane for the sums.  Bound by its
+// loads: every row and head reads its keys again, a lane's key value by value.  Four
+// sequences of 24 rows behind 1024..16384 tokens, 32 heads over 8 of width 80: 9.2 ms,
+// where the keys and values, read once, are 16 us.  It is there for widths that no
+// configuration of this framework has.
 __global__ void __launch_bounds__(64) tree_generic_kernel(const TreeCommon c) {
     extern __shared__ float sh[];
     const uint32_t D = c.head_dim, lane = threadIdx.x;
@@ -406,8 +410,8 @@ __global__ void __launch_bounds__(64) tree_generic_kernel(const TreeCommon c) {
 // of the wave, and the probabilities are in the layout of the next product's
 // operand where they are made.  q and p are split into bf16 parts that sum to
 // them: three of each (24 bits) for an f32 result; for a bf16 result two of q (its
-// rounding is multiplied by the scores' size) and one of p, whose rounding is no
-// larger than the result's own.  Products and sums are f32.
+// rounding is multiplied by the scores' size) and one of p, whose rounding is to the
+// values that it weighs what the result's is to the result.  Products and sums are f32.
 //
 // A workgroup has up to 4 x 32 query vectors and 32 KB stages of kKeys keys: a
 // wave takes one of the vector groups and 32 keys of a stage.  Stages come
@@ -419,10 +423,11 @@ __global__ void __launch_bounds__(64) tree_generic_kernel(const TreeCommon c) {
 // k - 1.
 //
 // What bounds it: the matrix pipe.  Eight sequences of 16..32 rows behind 1024..16384
-// tokens, 32 heads over 8 of width 128, f32: 120 us, of which 89 are its products at the
-// 1205 TFLOP/s that a large bf16 matrix product reaches, and 79 the loads alone.  Four
-// of 20..64 rows behind 8192..65536 tokens at width 256, bf16: 245 us; products 184, loads 74.
-// (Without its loads the kernel takes 93 and 226 us, with the loads alone 79 and 99.)
+// tokens, 32 heads over 8 of width 128, f32: 122 us (median of a kernel trace, one pass
+// after another), of which 89 are its products at the 1205 TFLOP/s that a large bf16
+// matrix product reaches, and 79 the loads alone.  Four of 20..64 rows behind 8192..65536
+// tokens at width 256, bf16: 251 us; products 184, loads 74.  (Without its loads the
+// kernel takes 93 and 226 us, with the loads alone 79 and 99.)
 // ---------------------------------------------------------------------------
 constexpr uint32_t kStages = 4;
 constexpr uint32_t kAhead = 2;  // stages on their way; one more may still be read by late waves
@@ -858,7 +863,7 @@ __global__ __launch_bounds__((TreeShape<D, kF32>::kThreads)) void tree_attn_kern
 }
 
 // Joins the records of a (row, head): a wave each, all the loads of eight records
-// in flight.  Bound by the records' bytes (32 MB in 8.9 us at width 256).
+// in flight.  Bound by the records' bytes (32 MB in 9.6 us at width 256).
 template <int D>
 __global__ void __launch_bounds__(256) tree_combine_kernel(const TreeCommon c, uint32_t rows) {
     constexpr int EPL = D / 64, kBatch = 8;

@@ -48,8 +48,10 @@ constexpr uint32_t tree_part_keys(uint32_t keys, uint32_t parts, uint32_t head_d
 }
 
 // Time of a key in tenths: one where every SIMD has two waves with query vectors.  With
-// fewer vectors it has one, which waits for itself: 1.7 against 2.45 us per stage at
-// head width 128.
+// fewer vectors it has one, with half the products but nothing beside it.  The 7 tenths are
+// by what the plan makes of eight sequences of unlike rows and contexts (160 -> 149 us);
+// with the same rows in every sequence, all CUs busy, a stage at width 128 takes 1.6 us
+// with 128 vectors and 1.4 with two (f32 result).
 inline uint32_t tree_key_cost(uint32_t head_dim, uint64_t vectors) {
     const uint32_t key_waves = tree_stage_keys(head_dim) / 32, vector_waves = tree_vector_waves(head_dim);
     const uint64_t tiles = std::min<uint64_t>(vector_waves, (vectors + kTreeVectors - 1) / kTreeVectors);
@@ -69,9 +71,12 @@ inline uint32_t tree_parts(const TreePlan &plan, uint32_t head_dim, uint32_t key
 
 // A workgroup fills its CU and costs its keys plus a start and an end, about 8 us; the
 // merge of records is 4.5 us and the writing and reading of them at 4 TB/s (17 / D^2 tenths
-// of a key per float).  A stage takes about D / 64 x 0.5 us (its products per wave go with
-// D), so that these are worth keys in inverse proportion to D^2: 300 tokens at width 256
-// take 21 us in partitions of two stages, 45 in one.  The candidates are the least budgets
+// of a key per float).  These are counted in keys as if a stage took D / 64 x 0.5 us, in
+// inverse proportion to D^2: 300 tokens at width 256 take 21 us in partitions of two
+// stages, 45 in one.  The stages measured with all CUs busy (128 vectors, 40 to 80 stages):
+// 2.3 us at width 64, 1.6 at 128, 1.7 at 256 for an f32 result, 1.4, 1.1 and 1.1 for bf16;
+// so the ends and the merge weigh up to four times what they take at width 64 and up to
+// twice at 128, for fewer and longer partitions.  The candidates are the least budgets
 // that make one to four rounds of workgroups over the CUs, and one partition per sequence.
 inline TreePlan tree_plan(uint32_t heads, uint32_t kv_heads, uint32_t head_dim,
                           uint32_t page_tokens, int num_cus, const SeqMeta *seqs, int nseq) {
