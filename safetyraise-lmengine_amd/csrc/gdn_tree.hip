@@ -764,10 +764,9 @@ template <int RT>
 hipError_t launch_head(hipStream_t stream, const GdnTreeParams &p) {
     using T = HeadShape<RT>;
     static_assert(T::kLds + 8192 <= 160 * 1024, "LDS");
-    static const hipError_t configured =
-        hipFuncSetAttribute((const void *)gdn_tree_head_kernel<RT>,
-                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)T::kLds);
-    if (configured != hipSuccess) return configured;
+    static LdsLimit limit;
+    const hipError_t e = limit.allow((const void *)gdn_tree_head_kernel<RT>, T::kLds);
+    if (e != hipSuccess) return e;
     SR_LAUNCH("gdn_tree_head_kernel", gdn_tree_head_kernel<RT>, dim3(p.value_heads, p.nseq), dim3(512),
               T::kLds, stream, p);
     return hipGetLastError();

@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 #include <exception>
@@ -276,6 +277,25 @@ int32_t no_throw(Ctx *ctx, F body) noexcept {
         }
     }
 }
+
+// Lets a kernel take `bytes` of dynamic LDS, above the default limit: an attribute that it
+// has on each device, set there before its first launch.
+class LdsLimit {
+  public:
+    hipError_t allow(const void *kernel, size_t bytes) {
+        int device = 0;
+        hipError_t e = hipGetDevice(&device);
+        if (e != hipSuccess) return e;
+        const uint64_t bit = (uint64_t)1 << (device & 63);
+        if (device < 64 && (devices_.load(std::memory_order_acquire) & bit) != 0) return hipSuccess;
+        e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+        if (e == hipSuccess && device < 64) devices_.fetch_or(bit, std::memory_order_release);
+        return e;
+    }
+
+  private:
+    std::atomic<uint64_t> devices_{0};
+};
 
 bool checked_mul(uint64_t a, uint64_t b, uint64_t *out);
 int32_t ensure_buffer(Ctx *ctx, DeviceBuffer &buf, size_t bytes, bool zero);

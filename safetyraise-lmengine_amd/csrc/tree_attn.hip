@@ -912,10 +912,9 @@ template <int D, bool kF32>
 hipError_t launch_attn(hipStream_t stream, const TreeCommon &c, uint32_t blocks) {
     using T = TreeShape<D, kF32>;
     static_assert(T::kLds <= 160 * 1024, "LDS");
-    static const hipError_t configured =
-        hipFuncSetAttribute((const void *)tree_attn_kernel<D, kF32>,
-                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)T::kLds);
-    if (configured != hipSuccess) return configured;
+    static LdsLimit limit;
+    const hipError_t e = limit.allow((const void *)tree_attn_kernel<D, kF32>, T::kLds);
+    if (e != hipSuccess) return e;
     SR_LAUNCH("tree_attn_kernel", (tree_attn_kernel<D, kF32>), dim3(blocks), dim3(T::kThreads),
               T::kLds, stream, c);
     return hipGetLastError();
