@@ -628,10 +628,11 @@ __global__ __launch_bounds__((TreeShape<D, kF32>::kThreads)) void tree_attn_kern
     // the beginning of step k
     auto enter = [&](uint32_t k) __attribute__((always_inline)) {
         // this wave's loads of stage k have landed when at most those of the
-        // stages after it are outstanding
+        // stages after it are outstanding; its reads of the stages before are done (the
+        // products that took them have waited for them, wherever the compiler put those)
         constexpr int kPer = 2 * kLoads < 64 ? 2 * kLoads : 63;
-        if (k + 1 < steps) __builtin_amdgcn_s_waitcnt(0x0F70 | (kPer & 15) | ((kPer >> 4) << 14));
-        else __builtin_amdgcn_s_waitcnt(0x0F70);
+        if (k + 1 < steps) __builtin_amdgcn_s_waitcnt(0x0070 | (kPer & 15) | ((kPer >> 4) << 14));
+        else __builtin_amdgcn_s_waitcnt(0x0070);
         // every wave's loads of stage k have landed, and the buffer of stage k - 2
         // has been read
         asm volatile("" ::: "memory");
