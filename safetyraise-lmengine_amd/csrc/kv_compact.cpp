@@ -44,7 +44,11 @@ int32_t upload_words(Ctx *ctx, size_t count, const uint32_t **device) {
     ctx->upload_next = (ctx->upload_next + 1) % kUploadSlots;
     SR_HIP(ctx, launch_linear_input(ctx->stream, (const float *)u.host_dev, (float *)u.dev.ptr,
                                     (count + 3) / 4 * 4));
-    SR_HIP(ctx, hipEventRecord(u.fetched, ctx->stream));
+    const hipError_t e = hipEventRecord(u.fetched, ctx->stream);
+    if (e != hipSuccess) {
+        (void)hipStreamSynchronize(ctx->stream);  // the slot's words are still being read
+        return hip_fail(ctx, e, "hipEventRecord");
+    }
     u.pending = true;
     *device = (const uint32_t *)u.dev.ptr;
     return kOk;

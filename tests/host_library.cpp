@@ -21,7 +21,7 @@ uint32_t random_below(uint32_t n) {
 }
 
 std::string g_fail;
-int g_fail_after = 0, g_null_copies = 0;
+int g_fail_after = 0, g_null_copies = 0, g_waits = 0;
 
 // a launch: an error where the test asks for one
 hipError_t launch(const char *name) {
@@ -63,6 +63,7 @@ void test_seed(uint64_t seed) { g_random = seed; }
 void test_fail(const char *name, int after) { g_fail = name, g_fail_after = after; }
 int test_failing() { return !g_fail.empty(); }
 int test_null_copies() { return g_null_copies; }
+int test_waits() { return g_waits; }
 
 void *__real_memcpy(void *to, const void *from, size_t n);
 void *__wrap_memcpy(void *to, const void *from, size_t n) {
@@ -114,7 +115,7 @@ const char *hipGetErrorName(hipError_t) { return "error"; }
 const char *hipGetErrorString(hipError_t) { return "a launch that the test made fail"; }
 hipError_t hipStreamCreate(hipStream_t *s) { return *s = (hipStream_t)std::malloc(1), hipSuccess; }
 hipError_t hipStreamDestroy(hipStream_t s) { return std::free((void *)s), hipSuccess; }
-hipError_t hipStreamSynchronize(hipStream_t) { return hipSuccess; }
+hipError_t hipStreamSynchronize(hipStream_t) { return ++g_waits, hipSuccess; }
 hipError_t hipStreamIsCapturing(hipStream_t, hipStreamCaptureStatus *c) {
     return *c = hipStreamCaptureStatusNone, hipSuccess;
 }
@@ -138,7 +139,7 @@ hipError_t hipMemcpyAsync(void *to, const void *from, size_t n, hipMemcpyKind k,
 hipError_t hipEventCreate(hipEvent_t *e) { return *e = (hipEvent_t)std::malloc(1), hipSuccess; }
 hipError_t hipEventCreateWithFlags(hipEvent_t *e, unsigned) { return hipEventCreate(e); }
 hipError_t hipEventDestroy(hipEvent_t e) { return std::free((void *)e), hipSuccess; }
-hipError_t hipEventRecord(hipEvent_t, hipStream_t) { return hipSuccess; }
+hipError_t hipEventRecord(hipEvent_t, hipStream_t) { return launch("event"); }
 hipError_t hipEventSynchronize(hipEvent_t) { return hipSuccess; }
 hipError_t hipEventElapsedTime(float *t, hipEvent_t, hipEvent_t) { return *t = 0, hipSuccess; }
 

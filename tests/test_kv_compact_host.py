@@ -316,6 +316,26 @@ def test_a_launch_that_fails_changes_nothing(host, launch):  # noqa: F811
     assert failed > 15
 
 
+def test_words_that_nothing_guards(host):  # noqa: F811
+    """Where the event that says when a call's words have been read cannot be recorded, they
+    are waited for: the next call may write over them."""
+    m = Model(host, pages=160)
+    a, b = m.new(900), m.new(500)
+    kept = [t for t in range(880) if t % 7]
+    entries = [(m, a, a, 20, kept), (m, b, b, 0, list(range(0, 500, 3)))]
+    for asynchronous in (False, True):
+        waits = host.test.test_waits()
+        host.test.test_fail(b"event", 0)
+        before = lists_of(m)
+        keeps = [(x.pool, *rest) for x, *rest in entries]
+        with pytest.raises(pkg.PluginError, match="hipEventRecord"):
+            pkg.kv_compact(host, keeps, asynchronous=asynchronous)
+        assert host.test.test_waits() > waits and lists_of(m) == before
+        m.check()
+    assert call(host, entries) == 0
+    m.check()
+
+
 def test_a_page_table_launch_that_fails(host):  # noqa: F811
     """The tokens have moved in place by then: the call reports the error, and the
     sequences are what it made them."""
