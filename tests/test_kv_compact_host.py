@@ -323,6 +323,9 @@ def test_words_that_nothing_guards(host):  # noqa: F811
     a, b = m.new(900), m.new(500)
     kept = [t for t in range(880) if t % 7]
     entries = [(m, a, a, 20, kept), (m, b, b, 0, list(range(0, 500, 3)))]
+    rows = [np.zeros((len(kept) * 2, KVH * DIM), np.float32) for _ in range(2)]
+    for _ in range(6):  # (memory for all the slots' words)
+        pkg.kv_gather(host, [(m.pool, a, 20, kept), (m.pool, a, 0, kept)], *rows)
     for asynchronous in (False, True):
         waits = host.test.test_waits()
         host.test.test_fail(b"event", 0)
