@@ -715,20 +715,29 @@ class _PoolMemory:
     """A pool on the device, held by its GdnState and by every tensor on its memory:
     freed when it has been given up (destroy) and the last of them is gone."""
 
+    waiting = []  # given up while a graph was captured, when nothing may be waited for or freed
+
     def __init__(self, backend: NativeBackend, handle):
         self.backend, self.handle = backend, handle
         self.given_up = False
-        self.viewed = None  # the device of the tensors on it, if there were any
+        self.viewed = None  # torch.cuda and the device of the tensors on it, if there were any
 
     def __del__(self):
-        if not self.given_up:
-            return
-        if self.viewed is not None:
-            # what reads it may still be queued on a stream of the caller's
-            import torch
+        if self.given_up:
+            self.waiting.append((self.backend, self.handle, self.viewed))
+            self.free_waiting()
 
-            torch.cuda.synchronize(self.viewed)
-        self.backend.lib.safetyraise_kernel_gdn_destroy(self.backend.context, self.handle)
+    @classmethod
+    def free_waiting(cls) -> None:
+        for _ in range(len(cls.waiting)):
+            backend, handle, viewed = cls.waiting.pop(0)
+            if viewed is not None:
+                cuda, device = viewed
+                if cuda.is_current_stream_capturing():
+                    cls.waiting.append((backend, handle, viewed))
+                    continue
+                cuda.synchronize(device)  # what reads it may still be queued on a stream of the caller's
+            backend.lib.safetyraise_kernel_gdn_destroy(backend.context, handle)
 
 
 class _DeviceArray:
@@ -770,6 +779,7 @@ class GdnState:
         backend.check(backend.lib.safetyraise_kernel_gdn_create(backend.context, C.byref(opts),
                                                                 C.byref(handle)), "gdn_create")
         self._memory = _PoolMemory(backend, handle)
+        _PoolMemory.free_waiting()
 
     @property
     def handle(self):
@@ -821,7 +831,8 @@ class GdnState:
         devices = [first] + [d for d in range(torch.cuda.device_count()) if d != first]
         state = _on_memory(_DeviceArray(self._memory, matrix.value, (
             self.value_heads, self.value_dim, self.key_dim)), devices)
-        device = self._memory.viewed = state.device
+        device = state.device
+        self._memory.viewed = torch.cuda, device
         history = _on_memory(_DeviceArray(self._memory, history.value, (
             self.channels, self.conv_kernel - 1)), [device.index])
         # (the default stream is behind the context's own one, which is a blocking one)
@@ -842,6 +853,7 @@ class GdnState:
         if self._memory is not None:
             self._memory.given_up = True
             self._memory = None
+        _PoolMemory.free_waiting()
 
 
 def gdn_forward(backend: NativeBackend, state: GdnState, seq_ids: Sequence[int],

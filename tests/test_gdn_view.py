@@ -106,6 +106,24 @@ def test_memory_stays_under_a_view(library):
     assert library.log.count("destroy 77") == 1
 
 
+def test_memory_given_up_under_capture(library):
+    """While a graph is captured nothing is waited for or freed: that is left to the next
+    pool that is made or destroyed."""
+    pool = new_pool(library)
+    views = pool.view(0)
+    pool.destroy()
+    library.capturing = True
+    del views
+    gc.collect()
+    assert "synchronize" not in library.log and "destroy 77" not in library.log
+    library.capturing = False
+    other = new_pool(library)
+    assert library.log[-2:] == ["synchronize", "destroy 77"]
+    library.log.clear()
+    other.destroy()
+    assert library.log == ["destroy 77"]
+
+
 def test_views_of_a_dropped_pool(library):
     """A pool object that is dropped without destroy leaves its memory."""
     state, history = new_pool(library).view(0)

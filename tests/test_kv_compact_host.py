@@ -113,7 +113,13 @@ def test_random_calls(host):  # noqa: F811
             elif op == 1 and len(m.held) < 9:
                 m.fork(s)
             elif op in (2, 3, 4):
-                m.append(s, int(rng.integers(1, 90)))
+                if rng.random() < 0.1:  # pages past its length, that hold nothing
+                    host.test.test_fail(b"kv_scatter", 0)
+                    with pytest.raises(pkg.PluginError):
+                        m.pool.append(s, *m.rows(int(rng.integers(1, 90))))
+                    host.test.test_fail(b"", 0)
+                else:
+                    m.append(s, int(rng.integers(1, 90)))
             elif op == 5 and len(m.held) > 4:
                 m.close(s)
             elif op == 6 and rng.random() < 0.3:
