@@ -445,7 +445,7 @@ SAFETYRAISE_KERNEL_EXPORT int32_t safetyraise_kernel_gdn_view(
  * Whole pages that stay whole at a page boundary are linked, not copied.
  * Pages shared with other sequences are never written: tokens that move
  * there go to free pages, OUT_OF_MEMORY (and nothing changed) when there are
- * too few.  Long moves without free pages are made in order, ten times slower.
+ * too few.  Long moves without free pages are made in order, several times slower.
  * A call that cannot be launched changes nothing either.  The tokens' values do not change (keys keep the RoPE position
  * they were written with).  Entries may name many pools (layers) and
  * sequences; no sequence may be the target of one entry and appear in
