@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(256) gdn_tree_generic_kernel(const GdnTreePara
 // inputs and state 7, conv and norms 6.3 (vector instructions: exponentials and
 // reciprocals of the silu; q and k are made once per value head of theirs), products 4.9,
 // solve 0.7, step 6 2.2 and 0.8 more for its checks of d, outputs 1.6.  One sequence of 12
-// rows: 10.7 us, mostly latency and the fetch of the code.  With 4-byte loads, the conv in place and the norms in a pass
-// of their own it took 32 us.
+// rows: 10.7 us, mostly latency and the fetch of the code.  With 4-byte loads, the conv in
+// place and the norms in a pass of their own it took 32 us.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kW = 128;         // Dk and Dv
 constexpr uint32_t kPitch = kW + 4;  // floats per LDS row (16 rows of 16 bytes meet no bank twice)

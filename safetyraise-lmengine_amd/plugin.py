@@ -736,7 +736,8 @@ class _PoolMemory:
                 if cuda.is_current_stream_capturing():
                     cls.waiting.append((backend, handle, viewed))
                     continue
-                cuda.synchronize(device)  # what reads it may still be queued on a stream of the caller's
+                # what reads it may still be queued on a stream of the caller's
+                cuda.synchronize(device)
             backend.lib.safetyraise_kernel_gdn_destroy(backend.context, handle)
 
 
